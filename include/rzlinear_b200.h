@@ -36,7 +36,7 @@ enum rz_status {
                                   every tensor-core launch on that device until rz_device_status has been called */
     RZ_ERR_UNSUPPORTED = -9,   /* the requested path cannot run this problem */
     RZ_ERR_TOO_LARGE = -10,    /* size exceeds a fixed capacity of the entry point */
-    RZ_ERR_SCRATCH = -11       /* the scratch buffer passed is smaller than rz_shadow_bytes() of the problem */
+    RZ_ERR_SCRATCH = -11       /* the scratch buffer passed is smaller than the size function of the entry point says */
 };
 
 enum rz_hash_mode {
@@ -178,6 +178,35 @@ int rz_device_status(int *out, int *detail);
    most `limit_cycles` SM cycles (1 .. 2e9) the wait gives up and the kernel returns; rz_device_status()
    then reports RZ_ERR_PIPELINE with detail 6, and the context stays usable. */
 int rz_selftest_bounded_wait(int64_t limit_cycles, void *stream);
+
+/* ---- rows picked by an index ------------------------------------------------------------------
+   No counterpart in the reference, whose only layer is RzLinear. */
+
+/* Stable counting sort of row keys: order[rows] = row numbers by ascending key, equal keys by ascending row;
+   offsets[bins + 1]: the rows of key b are order[offsets[b] .. offsets[b + 1]).  Rows whose key is outside [0, bins)
+   follow behind offsets[bins], in ascending order.  keys int64 [rows], order and offsets int32; 0 <= rows < 2^31,
+   1 <= bins <= RZ_SORT_MAX_BINS (RZ_ERR_TOO_LARGE beyond).  `scratch` (4-byte aligned) holds block histograms during the call:
+   rz_sort_rows_scratch_bytes() bytes, 0 for up to 2048 rows (then it may be NULL).  The result does not depend on
+   scheduling. */
+#define RZ_SORT_MAX_BINS 1024
+size_t rz_sort_rows_scratch_bytes(int64_t rows, int64_t bins);
+int rz_sort_rows(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order, int32_t *offsets, void *scratch,
+                 size_t scratch_bytes, void *stream);
+
+/* Embedding lookup in a virtual table W[K,N] of K rows: out[M,N] (io_dtype) = alpha * W[ids[m], :], read from the fp32
+   hashed array itself.  A token whose id is outside [0, K) or equal to padding_idx gives a row of zeros (pass a negative
+   padding_idx for none).  `precision` must go with io_dtype and is otherwise unused. */
+int rz_embedding_forward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const float *hashed, void *out,
+                         void *stream);
+
+/* Its gradient: dH[offset(k / BK, n / BN) + (k % BK) * BN + n % BN] += alpha * (sum of dOut[m, n] over the tokens with
+   ids[m] = k), fp32; dH is zeroed first unless RZ_FLAG_ACCUMULATE_DH.  Tokens that gave zeros contribute nothing, whatever
+   their dOut holds.  Tokens are sorted in chunks, and the rows of one token summed, before anything is added into dH; those additions
+   are fp32 reductions whose order is not fixed, as in rz_linear_backward_weight.  `scratch` (4-byte aligned):
+   rz_embedding_scratch_bytes() bytes during the call (0 for short batches; then it may be NULL). */
+size_t rz_embedding_scratch_bytes(const rz_problem *pb);
+int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const void *dOut, float *dH,
+                          void *scratch, size_t scratch_bytes, void *stream);
 
 /* Number of kernels this library has launched in this process (all threads). */
 uint64_t rz_launch_count(void);

@@ -30,7 +30,8 @@ EXPORTS = [
     "rz_linear_forward", "rz_linear_backward_input", "rz_linear_backward_weight",
     "rz_linear_materialize", "rz_sgd_step", "rz_device_status", "rz_launch_count",
     "rz_selftest_bounded_wait", "rz_sgd_momentum_step", "rz_grad_prepare", "rz_linear_forward_noalloc",
-    "rz_reload_env",
+    "rz_reload_env", "rz_sort_rows", "rz_sort_rows_scratch_bytes", "rz_embedding_forward",
+    "rz_embedding_scratch_bytes", "rz_embedding_backward",
 ]
 
 
@@ -91,12 +92,21 @@ def load() -> ctypes.CDLL:
         lib.rz_selftest_bounded_wait.argtypes = [ctypes.c_int64, vp]
         lib.rz_linear_forward_noalloc.argtypes = [pbp, vp, vp, vp, vp, vp]
         lib.rz_reload_env.restype = None
+        i64, sz = ctypes.c_int64, ctypes.c_size_t
+        lib.rz_sort_rows_scratch_bytes.argtypes = [i64, i64]
+        lib.rz_sort_rows_scratch_bytes.restype = sz
+        lib.rz_sort_rows.argtypes = [vp, i64, i64, vp, vp, vp, sz, vp]
+        lib.rz_embedding_forward.argtypes = [pbp, vp, i64, vp, vp, vp]
+        lib.rz_embedding_scratch_bytes.argtypes = [pbp]
+        lib.rz_embedding_scratch_bytes.restype = sz
+        lib.rz_embedding_backward.argtypes = [pbp, vp, i64, vp, vp, vp, sz, vp]
         lib.rz_device_status.argtypes = [ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]
         lib.rz_launch_count.restype = ctypes.c_uint64
         for name in ("rz_hash_indices_host", "rz_hash_indices_device", "rz_plan", "rz_shadow_refresh",
                      "rz_linear_forward", "rz_linear_backward_input", "rz_linear_backward_weight",
                      "rz_linear_materialize", "rz_sgd_step", "rz_device_status", "rz_sgd_momentum_step",
-                     "rz_selftest_bounded_wait", "rz_linear_forward_noalloc"):
+                     "rz_selftest_bounded_wait", "rz_linear_forward_noalloc", "rz_sort_rows", "rz_embedding_forward",
+                     "rz_embedding_backward"):
             getattr(lib, name).restype = ctypes.c_int
         _lib = lib
     return _lib
@@ -180,6 +190,18 @@ def _require_cuda(*tensors):
             raise RuntimeError("rzlinear_b200 kernels run on CUDA tensors only (there is no CPU path)")
 
 
+def _require_together(*tensors):
+    """CUDA tensors, all on one device."""
+    _require_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise RuntimeError(f"rzlinear_b200: tensors of one call must be on one device, got {sorted(map(str, devices))}")
+
+
+def _scratch(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def plan(pb: RzProblem, op: int) -> int:
     r = load().rz_plan(ctypes.byref(pb), op)
     if r < 0:
@@ -251,6 +273,32 @@ def grad_prepare(pb, dy, y, dym, bias_grad) -> None:
     _require_cuda(dy, y, dym, bias_grad)
     with _on(dy.device):
         check(load().rz_grad_prepare(ctypes.byref(pb), _ptr(dy), _ptr(y), _ptr(dym), _ptr(bias_grad), _stream(dy.device)))
+
+
+SORT_MAX_BINS = 1024
+
+
+def sort_rows(keys, bins, order, offsets) -> None:
+    """Stable counting sort of int64 row keys: see rz_sort_rows in include/rzlinear_b200.h."""
+    _require_together(keys, order, offsets)
+    scratch = _scratch(load().rz_sort_rows_scratch_bytes(keys.numel(), bins), keys.device)
+    with _on(keys.device):
+        check(load().rz_sort_rows(_ptr(keys), keys.numel(), bins, _ptr(order), _ptr(offsets), _ptr(scratch), _nbytes(scratch),
+                                  _stream(keys.device)))
+
+
+def embedding_forward(pb, ids, padding_idx, hashed, out) -> None:
+    _require_together(ids, hashed, out)
+    with _on(ids.device):
+        check(load().rz_embedding_forward(ctypes.byref(pb), _ptr(ids), padding_idx, _ptr(hashed), _ptr(out), _stream(ids.device)))
+
+
+def embedding_backward(pb, ids, padding_idx, dout, dh) -> None:
+    _require_together(ids, dout, dh)
+    scratch = _scratch(load().rz_embedding_scratch_bytes(ctypes.byref(pb)), ids.device)
+    with _on(ids.device):
+        check(load().rz_embedding_backward(ctypes.byref(pb), _ptr(ids), padding_idx, _ptr(dout), _ptr(dh), _ptr(scratch),
+                                           _nbytes(scratch), _stream(ids.device)))
 
 
 def sgd_step(pb, hashed, dh, lr, shadow) -> None:

@@ -11,11 +11,13 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "librzlinear_b200.so")
-SOURCES = ["rz_abi.cu", "rz_simt.cu", "rz_tc.cu", "rz_noalloc.cu", "rz_elementwise.cu"]
+SOURCES = ["rz_abi.cu", "rz_simt.cu", "rz_tc.cu", "rz_noalloc.cu", "rz_elementwise.cu", "rz_rows.cu"]
 HEADERS = ["rz_common.h", "rz_hash.h", "rz_ptx.cuh", os.path.join("..", "..", "include", "rzlinear_b200.h")]
 
 
@@ -37,16 +39,23 @@ def needs_build() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB_PATH
-    cmd = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-           "-Xcompiler", "-fPIC", "-shared", "-cudart", "shared",
-           "-Xlinker", "-rpath=/usr/local/cuda/lib64", "-o", LIB_PATH]
+    flags = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC"]
     if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += [os.path.join(CSRC, s) for s in SOURCES]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or proc.returncode:
-        sys.stderr.write(proc.stdout + proc.stderr)
-    if proc.returncode:
+        flags += ["-Xptxas", "-v"]
+
+    def run(args):
+        return subprocess.run([_nvcc()] + args, capture_output=True, text=True)
+
+    with tempfile.TemporaryDirectory() as tmp:   # one object per source, compiled side by side
+        objects = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            done = list(pool.map(run, [flags + ["-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objects)]))
+        if not any(p.returncode for p in done):
+            done.append(run(["-shared", "-cudart", "shared", "-Xlinker", "-rpath=/usr/local/cuda/lib64", "-o", LIB_PATH] + objects))
+    for proc in done:
+        if verbose or proc.returncode:
+            sys.stderr.write(proc.stdout + proc.stderr)
+    if any(p.returncode for p in done):
         raise RuntimeError("nvcc failed building librzlinear_b200.so")
     return LIB_PATH
 

@@ -69,6 +69,7 @@ RzHash make_hash(const rz_problem *pb)
     return h;
 }
 
+bool aligned_to(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 bool use_tc(const rz_problem *pb, int op)
@@ -85,6 +86,13 @@ RzLaunchCtx make_ctx(const rz_problem *pb, void *stream)
     c.hash = make_hash(pb);
     c.stream = reinterpret_cast<cudaStream_t>(stream);
     return c;
+}
+
+// dH = 0, unless the call adds into what is there
+int zero_gradient(const rz_problem *pb, float *dH, cudaStream_t stream)
+{
+    if (pb->flags & RZ_FLAG_ACCUMULATE_DH) return RZ_OK;
+    return rz_record_cuda(cudaMemsetAsync(dH, 0, sizeof(float) * (size_t)pb->H, stream), "zero dH");
 }
 
 }  // namespace
@@ -164,7 +172,7 @@ const char *rz_status_string(int status)
     case RZ_ERR_PIPELINE: return "device pipeline wait timed out (results since then are invalid; rz_device_status() clears it)";
     case RZ_ERR_UNSUPPORTED: return "problem not supported on the requested path";
     case RZ_ERR_TOO_LARGE: return "size exceeds the capacity of this entry point";
-    case RZ_ERR_SCRATCH: return "scratch buffer smaller than rz_shadow_bytes() of this problem";
+    case RZ_ERR_SCRATCH: return "scratch buffer smaller than rz_shadow_bytes() (or the entry point's own size function) of this problem";
     default: return "unknown status";
     }
 }
@@ -245,10 +253,8 @@ int rz_linear_backward_weight(const rz_problem *pb, const void *X, const void *d
     if (st) return st;
     if (!X || !dY || !dH) return RZ_ERR_NULL;
     RzLaunchCtx c = make_ctx(pb, stream);
-    if (!(pb->flags & RZ_FLAG_ACCUMULATE_DH)) {
-        st = rz_record_cuda(cudaMemsetAsync(dH, 0, sizeof(float) * (size_t)pb->H, c.stream), "zero dH");
-        if (st) return st;
-    }
+    st = zero_gradient(pb, dH, c.stream);
+    if (st) return st;
     if (use_tc(pb, RZ_OP_BACKWARD_WEIGHT)) {
         if (!aligned16(X) || !aligned16(dY) || !aligned16(dH)) return RZ_ERR_ALIGN;
         return rz_tc_backward_weight(c, X, dY, dH);
@@ -270,6 +276,53 @@ int rz_grad_prepare(const rz_problem *pb, const void *dY, const void *Y, void *d
     if (st) return st;
     if (!dY || (Y && !dYm) || (!dYm && !bias_grad)) return RZ_ERR_NULL;
     return rz_elementwise_grad_prepare(make_ctx(pb, stream), dY, Y, dYm, bias_grad);
+}
+
+size_t rz_sort_rows_scratch_bytes(int64_t rows, int64_t bins)
+{
+    if (rows < 0 || rows >= ((int64_t)1 << 31) || bins <= 0 || bins > RZ_SORT_MAX_BINS) return 0;
+    return rz_rows_sort_scratch(rows, bins);
+}
+
+int rz_sort_rows(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order, int32_t *offsets, void *scratch,
+                 size_t scratch_bytes, void *stream)
+{
+    if (rows < 0 || rows >= ((int64_t)1 << 31) || bins <= 0) return RZ_ERR_SHAPE;
+    if (bins > RZ_SORT_MAX_BINS) return RZ_ERR_TOO_LARGE;
+    if (!offsets || (rows > 0 && (!keys || !order))) return RZ_ERR_NULL;
+    const size_t need = rz_rows_sort_scratch(rows, bins);
+    if (need && !scratch) return RZ_ERR_NULL;
+    if (scratch_bytes < need) return RZ_ERR_SCRATCH;
+    if (!aligned_to(keys, 8) || !aligned_to(order, 4) || !aligned_to(offsets, 4) || !aligned_to(scratch, 4)) return RZ_ERR_ALIGN;
+    return rz_rows_sort(keys, rows, bins, order, offsets, scratch, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int rz_embedding_forward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const float *hashed, void *out, void *stream)
+{
+    int st = validate(pb);
+    if (st) return st;
+    if (!ids || !hashed || !out) return RZ_ERR_NULL;
+    if (!aligned_to(ids, 8) || !aligned_to(hashed, 4) || !aligned_to(out, pb->io_dtype == RZ_BF16 ? 2 : 4)) return RZ_ERR_ALIGN;
+    return rz_rows_embedding(make_ctx(pb, stream), ids, padding_idx, hashed, out);
+}
+
+size_t rz_embedding_scratch_bytes(const rz_problem *pb) { return validate(pb) ? 0 : rz_rows_embedding_scratch(pb); }
+
+int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const void *dOut, float *dH, void *scratch,
+                          size_t scratch_bytes, void *stream)
+{
+    int st = validate(pb);
+    if (st) return st;
+    if (!ids || !dOut || !dH) return RZ_ERR_NULL;
+    const size_t need = rz_rows_embedding_scratch(pb);
+    if (need && !scratch) return RZ_ERR_NULL;
+    if (scratch_bytes < need) return RZ_ERR_SCRATCH;
+    if (!aligned_to(ids, 8) || !aligned_to(dOut, pb->io_dtype == RZ_BF16 ? 2 : 4) || !aligned_to(dH, 4) || !aligned_to(scratch, 4))
+        return RZ_ERR_ALIGN;
+    RzLaunchCtx c = make_ctx(pb, stream);
+    st = zero_gradient(pb, dH, c.stream);
+    if (st) return st;
+    return rz_rows_embedding_grad(c, ids, padding_idx, dOut, dH, scratch);
 }
 
 int rz_sgd_step(const rz_problem *pb, float *hashed, const float *dH, float lr, void *shadow, void *stream)

@@ -72,3 +72,11 @@ int rz_tc_forward(const RzLaunchCtx &c, const void *X, void *shadow, size_t shad
 int rz_tc_backward_input(const RzLaunchCtx &c, const void *dY, void *shadow, size_t shadow_bytes, void *dX);
 int rz_tc_backward_weight(const RzLaunchCtx &c, const void *X, const void *dY, float *dH);
 int rz_tc_wait_selftest(long long limit_cycles, cudaStream_t stream);
+
+// rows picked by an index (rz_rows.cu): M = rows or tokens, K = table rows, N = row length
+size_t rz_rows_sort_scratch(int64_t rows, int64_t bins);
+int rz_rows_sort_max_bins();
+int rz_rows_sort(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order, int32_t *offsets, void *scratch, cudaStream_t stream);
+int rz_rows_embedding(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const float *hashed, void *out);
+size_t rz_rows_embedding_scratch(const rz_problem *pb);
+int rz_rows_embedding_grad(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const void *dout, float *dH, void *scratch);
