@@ -208,6 +208,42 @@ size_t rz_embedding_scratch_bytes(const rz_problem *pb);
 int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const void *dOut, float *dH,
                           void *scratch, size_t scratch_bytes, void *stream);
 
+/* ---- products grouped by row (the experts of a layer) -----------------------------------------
+   M rows in `groups` consecutive groups: rows offsets[g] .. offsets[g + 1) belong to group g (int32 [groups + 1], on the device; the
+   host never reads it).  Every group has a K x N weight of its own; they are one virtual matrix, one below the other, each beginning
+   with a new tile row: W_g[k,n] = hashed[ offset(g * ceil(K/BK) + k / BK, n / BN) + (k % BK) * BN + n % BN ].  Groups may be
+   empty.  Rows before offsets[0] and behind the last offset belong to no group: their results are zeros and they add to no gradient.
+   Offsets outside [0, M] count as the nearer end and an offset below an earlier one as that one, so no call reads or writes out of
+   range.  1 <= groups <= RZ_GROUPS_LIMIT (RZ_ERR_TOO_LARGE beyond), groups * ceil(K/BK) * BK < 2^31.  Shapes, types and precisions are
+   rz_linear_forward's, and rz_plan() says which kernels run (fp32 precision with K or N above 14336 runs the FMA kernels here).
+
+   `copies`: the shifted copies that rz_shadow_refresh writes (rz_grouped_copies_bytes() of them, 0 on the SIMT path; a shadow
+   buffer of rz_linear_forward with the same H and precision serves too); only read, so calls may share them.  `workspace`
+   (256-byte aligned, rz_grouped_workspace_bytes()): written by the call, so calls that may overlap need one each. */
+#define RZ_GROUPS_LIMIT 4096
+size_t rz_grouped_copies_bytes(const rz_problem *pb);
+size_t rz_grouped_workspace_bytes(const rz_problem *pb, int64_t groups);
+
+/* Y[r,:] = alpha * X[r,:] . W_g (+ bias[g,:], fp32 [groups, N], may be NULL) (+ ReLU with RZ_FLAG_RELU) for r in group g. */
+int rz_grouped_forward(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const float *hashed,
+                       const void *copies, size_t copies_bytes, const float *bias, void *Y, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
+/* dX[r,:] = alpha * dY[r,:] . W_g^T. */
+int rz_grouped_backward_input(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *dY, const float *hashed,
+                              const void *copies, size_t copies_bytes, void *dX, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
+/* dH[word of W_g[k,n]] += alpha * sum over the rows r of group g of X[r,k] dY[r,n], for every group; dH is zeroed first unless
+   RZ_FLAG_ACCUMULATE_DH. */
+int rz_grouped_backward_weight(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const void *dY, float *dH,
+                               void *workspace, size_t workspace_bytes, void *stream);
+
+/* rz_grad_prepare with a bias for each group: bias_grad fp32 [groups, N].  Rows of dYm that belong to no group are not written
+   (the grouped calls do not look at them). */
+int rz_grouped_grad_prepare(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *dY, const void *Y, void *dYm,
+                            float *bias_grad, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Number of kernels this library has launched in this process (all threads). */
 uint64_t rz_launch_count(void);
 

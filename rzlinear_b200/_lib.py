@@ -31,7 +31,8 @@ EXPORTS = [
     "rz_linear_materialize", "rz_sgd_step", "rz_device_status", "rz_launch_count",
     "rz_selftest_bounded_wait", "rz_sgd_momentum_step", "rz_grad_prepare", "rz_linear_forward_noalloc",
     "rz_reload_env", "rz_sort_rows", "rz_sort_rows_scratch_bytes", "rz_embedding_forward",
-    "rz_embedding_scratch_bytes", "rz_embedding_backward",
+    "rz_embedding_scratch_bytes", "rz_embedding_backward", "rz_grouped_copies_bytes", "rz_grouped_workspace_bytes",
+    "rz_grouped_forward", "rz_grouped_backward_input", "rz_grouped_backward_weight", "rz_grouped_grad_prepare",
 ]
 
 
@@ -100,13 +101,22 @@ def load() -> ctypes.CDLL:
         lib.rz_embedding_scratch_bytes.argtypes = [pbp]
         lib.rz_embedding_scratch_bytes.restype = sz
         lib.rz_embedding_backward.argtypes = [pbp, vp, i64, vp, vp, vp, sz, vp]
+        lib.rz_grouped_copies_bytes.argtypes = [pbp]
+        lib.rz_grouped_copies_bytes.restype = sz
+        lib.rz_grouped_workspace_bytes.argtypes = [pbp, i64]
+        lib.rz_grouped_workspace_bytes.restype = sz
+        lib.rz_grouped_forward.argtypes = [pbp, i64, vp, vp, vp, vp, sz, vp, vp, vp, sz, vp]
+        lib.rz_grouped_backward_input.argtypes = [pbp, i64, vp, vp, vp, vp, sz, vp, vp, sz, vp]
+        lib.rz_grouped_backward_weight.argtypes = [pbp, i64, vp, vp, vp, vp, vp, sz, vp]
+        lib.rz_grouped_grad_prepare.argtypes = [pbp, i64, vp, vp, vp, vp, vp, vp, sz, vp]
         lib.rz_device_status.argtypes = [ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]
         lib.rz_launch_count.restype = ctypes.c_uint64
         for name in ("rz_hash_indices_host", "rz_hash_indices_device", "rz_plan", "rz_shadow_refresh",
                      "rz_linear_forward", "rz_linear_backward_input", "rz_linear_backward_weight",
                      "rz_linear_materialize", "rz_sgd_step", "rz_device_status", "rz_sgd_momentum_step",
                      "rz_selftest_bounded_wait", "rz_linear_forward_noalloc", "rz_sort_rows", "rz_embedding_forward",
-                     "rz_embedding_backward"):
+                     "rz_embedding_backward", "rz_grouped_forward", "rz_grouped_backward_input", "rz_grouped_backward_weight",
+                     "rz_grouped_grad_prepare"):
             getattr(lib, name).restype = ctypes.c_int
         _lib = lib
     return _lib
@@ -299,6 +309,45 @@ def embedding_backward(pb, ids, padding_idx, dout, dh) -> None:
     with _on(ids.device):
         check(load().rz_embedding_backward(ctypes.byref(pb), _ptr(ids), padding_idx, _ptr(dout), _ptr(dh), _ptr(scratch),
                                            _nbytes(scratch), _stream(ids.device)))
+
+
+def grouped_copies_bytes(pb) -> int:
+    return int(load().rz_grouped_copies_bytes(ctypes.byref(pb)))
+
+
+def grouped_workspace(pb, groups: int, device):
+    """Workspace for the grouped calls of one stream; raises for a problem that rz_grouped_* would refuse."""
+    nbytes = int(load().rz_grouped_workspace_bytes(ctypes.byref(pb), groups))
+    return _scratch(max(nbytes, 256), device)
+
+
+def grouped_forward(pb, groups, offsets, x, hashed, copies, bias, y, ws) -> None:
+    _require_together(offsets, x, hashed, copies, bias, y, ws)
+    with _on(x.device):
+        check(load().rz_grouped_forward(ctypes.byref(pb), groups, _ptr(offsets), _ptr(x), _ptr(hashed), _ptr(copies), _nbytes(copies),
+                                        _ptr(bias), _ptr(y), _ptr(ws), _nbytes(ws), _stream(x.device)))
+
+
+def grouped_backward_input(pb, groups, offsets, dy, hashed, copies, dx, ws) -> None:
+    _require_together(offsets, dy, hashed, copies, dx, ws)
+    with _on(dy.device):
+        check(load().rz_grouped_backward_input(ctypes.byref(pb), groups, _ptr(offsets), _ptr(dy), _ptr(hashed), _ptr(copies),
+                                               _nbytes(copies), _ptr(dx), _ptr(ws), _nbytes(ws), _stream(dy.device)))
+
+
+def grouped_backward_weight(pb, groups, offsets, x, dy, dh, ws) -> None:
+    _require_together(offsets, x, dy, dh, ws)
+    with _on(x.device):
+        check(load().rz_grouped_backward_weight(ctypes.byref(pb), groups, _ptr(offsets), _ptr(x), _ptr(dy), _ptr(dh), _ptr(ws),
+                                                _nbytes(ws), _stream(x.device)))
+
+
+def grouped_grad_prepare(pb, groups, offsets, dy, y, dym, bias_grad, ws) -> None:
+    """dym = dy where y > 0 (y may be None), bias_grad[g] = column sums of group g's (masked) gradient (may be None)."""
+    _require_together(offsets, dy, y, dym, bias_grad, ws)
+    with _on(dy.device):
+        check(load().rz_grouped_grad_prepare(ctypes.byref(pb), groups, _ptr(offsets), _ptr(dy), _ptr(y), _ptr(dym), _ptr(bias_grad),
+                                             _ptr(ws), _nbytes(ws), _stream(dy.device)))
 
 
 def sgd_step(pb, hashed, dh, lr, shadow) -> None:

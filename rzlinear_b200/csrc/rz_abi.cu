@@ -69,6 +69,17 @@ RzHash make_hash(const rz_problem *pb)
     return h;
 }
 
+// `groups` weights of K x N, one below the other in one virtual matrix, every one beginning with a new tile row
+int validate_groups(const rz_problem *pb, int64_t groups)
+{
+    int st = validate(pb);
+    if (st) return st;
+    if (groups <= 0) return RZ_ERR_SHAPE;
+    if (groups > RZ_GROUPS_MAX) return RZ_ERR_TOO_LARGE;
+    const int64_t tile_rows = groups * ((pb->K + pb->BK - 1) / pb->BK);
+    return tile_rows * pb->BK >= ((int64_t)1 << 31) ? RZ_ERR_SHAPE : RZ_OK;
+}
+
 bool aligned_to(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -86,6 +97,29 @@ RzLaunchCtx make_ctx(const rz_problem *pb, void *stream)
     c.hash = make_hash(pb);
     c.stream = reinterpret_cast<cudaStream_t>(stream);
     return c;
+}
+
+// Grouped launches in split precision have seven accumulation chains at most: beyond 2048 elements each (6e-6 of truncation) the FMA
+// kernels run.
+bool use_tc_grouped(const rz_problem *pb)
+{
+    if (pb->precision == RZ_PREC_FP32 && (pb->K > 7 * 2048 || pb->N > 7 * 2048)) return false;
+    return use_tc(pb, RZ_OP_FORWARD);   // (the same for all three operations)
+}
+
+// What the grouped entry points ask of their buffers besides that they exist.
+int check_grouped(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *in, const void *out, const void *copies,
+                  size_t copies_bytes, const void *workspace, size_t workspace_bytes, bool tc, bool needs_copies = true)
+{
+    if (!offsets || !workspace) return RZ_ERR_NULL;
+    const uintptr_t element = pb->io_dtype == RZ_BF16 ? 2 : 4;
+    if (!aligned_to(offsets, 4) || !aligned_to(workspace, 256) || !aligned_to(in, tc ? 16 : element) || !aligned_to(out, tc ? 16 : element))
+        return RZ_ERR_ALIGN;
+    if (tc && needs_copies) {
+        if (!aligned_to(copies, 256)) return RZ_ERR_ALIGN;
+        if (copies_bytes < rz_tc_copies_bytes(pb)) return RZ_ERR_SCRATCH;
+    }
+    return workspace_bytes < rz_grouped_workspace(pb, (int)groups, use_tc_grouped(pb)) ? RZ_ERR_SCRATCH : RZ_OK;
 }
 
 // dH = 0, unless the call adds into what is there
@@ -323,6 +357,70 @@ int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padd
     st = zero_gradient(pb, dH, c.stream);
     if (st) return st;
     return rz_rows_embedding_grad(c, ids, padding_idx, dOut, dH, scratch);
+}
+
+size_t rz_grouped_copies_bytes(const rz_problem *pb)
+{
+    if (validate(pb)) return 0;
+    return use_tc_grouped(pb) ? rz_tc_copies_bytes(pb) : 0;
+}
+
+size_t rz_grouped_workspace_bytes(const rz_problem *pb, int64_t groups)
+{
+    if (validate_groups(pb, groups)) return 0;
+    return rz_grouped_workspace(pb, (int)groups, use_tc_grouped(pb));
+}
+
+int rz_grouped_forward(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const float *hashed, const void *copies,
+                       size_t copies_bytes, const float *bias, void *Y, void *workspace, size_t workspace_bytes, void *stream)
+{
+    int st = validate_groups(pb, groups);
+    if (st) return st;
+    const bool tc = use_tc_grouped(pb);
+    if (!X || !Y || (tc ? !copies : !hashed)) return RZ_ERR_NULL;
+    st = check_grouped(pb, groups, offsets, X, Y, copies, copies_bytes, workspace, workspace_bytes, tc);
+    if (st) return st;
+    return rz_grouped_run_forward(make_ctx(pb, stream), (int)groups, offsets, X, hashed, copies, bias, Y, workspace, tc);
+}
+
+int rz_grouped_backward_input(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *dY, const float *hashed,
+                              const void *copies, size_t copies_bytes, void *dX, void *workspace, size_t workspace_bytes, void *stream)
+{
+    int st = validate_groups(pb, groups);
+    if (st) return st;
+    const bool tc = use_tc_grouped(pb);
+    if (!dY || !dX || (tc ? !copies : !hashed)) return RZ_ERR_NULL;
+    st = check_grouped(pb, groups, offsets, dY, dX, copies, copies_bytes, workspace, workspace_bytes, tc);
+    if (st) return st;
+    return rz_grouped_run_backward_input(make_ctx(pb, stream), (int)groups, offsets, dY, hashed, copies, dX, workspace, tc);
+}
+
+int rz_grouped_backward_weight(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const void *dY, float *dH,
+                               void *workspace, size_t workspace_bytes, void *stream)
+{
+    int st = validate_groups(pb, groups);
+    if (st) return st;
+    if (!X || !dY || !dH) return RZ_ERR_NULL;
+    if (!aligned_to(dH, 4)) return RZ_ERR_ALIGN;
+    const bool tc = use_tc_grouped(pb);
+    st = check_grouped(pb, groups, offsets, X, dY, nullptr, 0, workspace, workspace_bytes, tc, false);
+    if (st) return st;
+    RzLaunchCtx c = make_ctx(pb, stream);
+    st = zero_gradient(pb, dH, c.stream);
+    if (st) return st;
+    return rz_grouped_run_backward_weight(c, (int)groups, offsets, X, dY, dH, workspace, tc);
+}
+
+int rz_grouped_grad_prepare(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *dY, const void *Y, void *dYm,
+                            float *bias_grad, void *workspace, size_t workspace_bytes, void *stream)
+{
+    int st = validate_groups(pb, groups);
+    if (st) return st;
+    if (!dY || (Y && !dYm) || (!dYm && !bias_grad)) return RZ_ERR_NULL;
+    if (!aligned_to(bias_grad, 4)) return RZ_ERR_ALIGN;
+    st = check_grouped(pb, groups, offsets, dY, Y, nullptr, 0, workspace, workspace_bytes, false, false);
+    if (st) return st;
+    return rz_grouped_run_grad_prepare(make_ctx(pb, stream), (int)groups, offsets, dY, Y, dYm, bias_grad, workspace);
 }
 
 int rz_sgd_step(const rz_problem *pb, float *hashed, const float *dH, float lr, void *shadow, void *stream)

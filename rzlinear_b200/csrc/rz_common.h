@@ -37,6 +37,14 @@ struct RzLaunchCtx {
     cudaStream_t stream;
 };
 
+// Pieces of a grouped launch: consecutive rows of one group, as the plan kernel lists them on the device.
+struct RzGroupPieces {
+    const uint32_t *header = nullptr;   // [0] = how many there are
+    const uint4 *entries = nullptr;     // {group, first row, end, 0}
+    uint32_t most = 0;                  // the host's bound on header[0]
+    uint32_t group_tiles = 0;           // hash-tile rows of one group's weight
+};
+
 // host helpers (rz_abi.cu)
 int rz_record_cuda(cudaError_t e, const char *what);
 void rz_count_launch(int n);
@@ -80,3 +88,32 @@ int rz_rows_sort(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order
 int rz_rows_embedding(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const float *hashed, void *out);
 size_t rz_rows_embedding_scratch(const rz_problem *pb);
 int rz_rows_embedding_grad(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const void *dout, float *dH, void *scratch);
+
+// products grouped by row (rz_grouped.cu): pb->M rows in `groups` consecutive groups given by offsets[groups + 1] on the device
+constexpr int RZ_GROUPS_MAX = 4096;
+size_t rz_grouped_workspace(const rz_problem *pb, int groups, bool tc);
+int rz_grouped_run_forward(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *X, const float *hashed, const void *copies,
+                           const float *bias, void *Y, void *ws, bool tc);
+int rz_grouped_run_backward_input(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *dY, const float *hashed,
+                                  const void *copies, void *dX, void *ws, bool tc);
+int rz_grouped_run_backward_weight(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *X, const void *dY, float *dH,
+                                   void *ws, bool tc);
+int rz_grouped_run_grad_prepare(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *dY, const void *Y, void *dYm,
+                                float *bias_grad, void *ws);
+
+int rz_simt_grouped_forward(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *X, const float *hashed, const float *bias, void *Y);
+int rz_simt_grouped_backward_input(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *dY, const float *hashed, void *dX);
+int rz_simt_grouped_backward_weight(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *X, const void *dY, float *dH);
+
+// tensor-core launches of a grouped operation (rz_tc_grouped.cu)
+struct RzTcGroupPlan {
+    int ctas, rb, nc, ew;   // block shape
+    uint32_t step;          // most rows of a piece
+};
+RzTcGroupPlan rz_tc_grouped_plan(const rz_problem *pb, int groups, int op);
+int rz_tc_grouped_forward(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *X, const void *copies,
+                          const float *bias, void *Y);
+int rz_tc_grouped_backward_input(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *dY,
+                                 const void *copies, void *dX);
+// `maps`: {dY, X} tensor maps of each group on the device, made from rz_tc_grouped_base_maps() by the plan kernel
+int rz_tc_grouped_backward_weight(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *maps, float *dH);

@@ -119,6 +119,24 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap *map)
 {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
+// Makes a tensor map that a kernel wrote to global memory visible to this thread's TMA instructions.
+__device__ __forceinline__ void tma_acquire_desc(const CUtensorMap *map)
+{
+    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+// Replaces the extent of dimension 1 (rows) of a tensor map in shared memory.
+__device__ __forceinline__ void tma_replace_rows(uint32_t map_smem, uint32_t rows)
+{
+    asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"r"(map_smem), "r"(rows) : "memory");
+}
+// Publishes a tensor map from shared to global memory (whole warp).
+__device__ __forceinline__ void tma_publish_desc(CUtensorMap *dst, uint32_t src_smem)
+{
+    asm volatile("tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned [%0], [%1], 128;" ::"l"(
+                     reinterpret_cast<uint64_t>(dst)),
+                 "r"(src_smem)
+                 : "memory");
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t x, int32_t y)
 {
     asm volatile(

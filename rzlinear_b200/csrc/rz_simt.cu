@@ -46,23 +46,26 @@ struct TileMemo {
 // TB: block edge (64 or 128).  A thread owns G x G groups of 4 x 4 outputs, G = TB / 64, the groups 64 apart, so
 // that its shared-memory reads are 16-byte loads without bank conflicts.  TC * TB = 1024: four elements of either
 // operand per thread and chunk.
-template <int OP, typename T, int TB>
+// GROUPED: the rows come in groups with a weight each (rz_grouped.cu).  blockIdx.x is a piece {group, first row, end}: the rows of
+// the output block (OP 0, 1) or the contraction (OP 2); the block's columns are blockIdx.y's, OP 2's rows blockIdx.z's.
+template <int OP, typename T, int TB, int GROUPED = 0>
 __global__ void __launch_bounds__(256)
 rz_simt_kernel(const T *__restrict__ A, const T *__restrict__ B2, const float *__restrict__ hashed,
                const float *__restrict__ bias, void *__restrict__ out_, float *__restrict__ dH,
-               RzHash hash, uint32_t M, uint32_t K, uint32_t N, float alpha, int relu, uint32_t chunk_per_split)
+               RzHash hash, uint32_t M, uint32_t K, uint32_t N, float alpha, int relu, uint32_t chunk_per_split,
+               RzGroupPieces pieces = RzGroupPieces())
 {
     constexpr int TC = 1024 / TB;   // contraction chunk: 16 (TB = 64) or 8 (TB = 128)
     constexpr int G = TB / 64;
     __shared__ __align__(16) float As[2][TC][TB + PAD];
     __shared__ __align__(16) float Bs[2][TC][TB + PAD];
 
-    const uint32_t rows = (OP == 2) ? K : M;
+    uint32_t rows = (OP == 2) ? K : M;
     const uint32_t cols = (OP == 1) ? K : N;
     const uint32_t depth = (OP == 0) ? K : (OP == 1 ? N : M);
 
-    const uint32_t r0 = blockIdx.y * TB;
-    const uint32_t c0 = blockIdx.x * TB;
+    uint32_t r0 = blockIdx.y * TB, c0 = blockIdx.x * TB;
+    uint32_t k_base = 0;   // first row of the group's weight in the stacked virtual matrix
     const uint32_t tid = threadIdx.x;
     const uint32_t tx = tid % 16, ty = tid / 16;
 
@@ -70,6 +73,19 @@ rz_simt_kernel(const T *__restrict__ A, const T *__restrict__ B2, const float *_
     if (OP == 2) {
         d_begin = blockIdx.z * chunk_per_split;
         d_end = min(depth, d_begin + chunk_per_split);
+    }
+    if (GROUPED) {
+        if (blockIdx.x >= __ldg(pieces.header)) return;
+        const uint4 piece = __ldg(pieces.entries + blockIdx.x);
+        k_base = piece.x * pieces.group_tiles * (uint32_t)hash.BK;
+        c0 = blockIdx.y * TB;
+        if (OP == 2) {
+            r0 = blockIdx.z * TB;
+            d_begin = piece.y, d_end = piece.z;
+        } else {
+            r0 = piece.y, rows = piece.z;
+            if (OP == 0 && bias) bias += (size_t)piece.x * N;
+        }
     }
 
     float acc[4 * G][4 * G];
@@ -107,14 +123,14 @@ rz_simt_kernel(const T *__restrict__ A, const T *__restrict__ B2, const float *_
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t n = c0 + e4_of + e;
-                rb[e] = (k < d_end && n < cols) ? hashed[memo.index(hash, k, n)] : 0.f;
+                rb[e] = (k < d_end && n < cols) ? hashed[memo.index(hash, k_base + k, n)] : 0.f;
             }
         } else if (OP == 1) {       // B(n, k) = W[k][n]: contiguous along the contraction n
             const uint32_t k = c0 + x_of;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t n = d0 + d4_of + e;
-                rb[e] = (k < cols && n < d_end) ? hashed[memo.index(hash, k, n)] : 0.f;
+                rb[e] = (k < cols && n < d_end) ? hashed[memo.index(hash, k_base + k, n)] : 0.f;
             }
         } else {                    // B(m, n) = dY[m][n]
             const uint32_t m = d0 + dd_of;
@@ -177,7 +193,7 @@ rz_simt_kernel(const T *__restrict__ A, const T *__restrict__ B2, const float *_
 #pragma unroll
             for (int j = 0; j < 4 * G; ++j) {
                 const uint32_t k = r0 + (i / 4) * 64 + ty * 4 + (i % 4), n = c0 + (j / 4) * 64 + tx * 4 + (j % 4);
-                if (k < rows && n < cols) atomicAdd(dH + em.index(hash, k, n), acc[i][j] * alpha);
+                if (k < rows && n < cols) atomicAdd(dH + em.index(hash, k_base + k, n), acc[i][j] * alpha);
             }
     } else {
         T *out = reinterpret_cast<T *>(out_);
@@ -262,7 +278,42 @@ int launch(const RzLaunchCtx &c, const void *A, const void *B2, const float *has
     return launch_block<OP, 64>(c, A, B2, hashed, bias, out, dH);
 }
 
+template <int OP>
+int launch_grouped(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *A, const void *B2, const float *hashed,
+                   const float *bias, void *out, float *dH)
+{
+    const rz_problem *pb = c.pb;
+    const uint32_t M = (uint32_t)pb->M, K = (uint32_t)pb->K, N = (uint32_t)pb->N;
+    const uint32_t cols = (OP == 1) ? K : N;
+    const dim3 grid(pieces.most, (cols + 63) / 64, OP == 2 ? (K + 63) / 64 : 1);
+    if (grid.y > 65535u || grid.z > 65535u) return RZ_ERR_SHAPE;
+    const int relu = (pb->flags & RZ_FLAG_RELU) ? 1 : 0;
+    if (pb->io_dtype == RZ_F32)
+        rz_simt_kernel<OP, float, 64, 1><<<grid, 256, 0, c.stream>>>((const float *)A, (const float *)B2, hashed, bias, out, dH, c.hash,
+                                                                    M, K, N, pb->alpha, relu, 0, pieces);
+    else
+        rz_simt_kernel<OP, __nv_bfloat16, 64, 1><<<grid, 256, 0, c.stream>>>((const __nv_bfloat16 *)A, (const __nv_bfloat16 *)B2, hashed,
+                                                                            bias, out, dH, c.hash, M, K, N, pb->alpha, relu, 0, pieces);
+    rz_count_launch(1);
+    return rz_record_cuda(cudaGetLastError(), "grouped simt launch");
+}
+
 }  // namespace
+
+int rz_simt_grouped_forward(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *X, const float *hashed, const float *bias, void *Y)
+{
+    return launch_grouped<0>(c, pieces, X, nullptr, hashed, bias, Y, nullptr);
+}
+
+int rz_simt_grouped_backward_input(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *dY, const float *hashed, void *dX)
+{
+    return launch_grouped<1>(c, pieces, dY, nullptr, hashed, nullptr, dX, nullptr);
+}
+
+int rz_simt_grouped_backward_weight(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *X, const void *dY, float *dH)
+{
+    return launch_grouped<2>(c, pieces, X, dY, nullptr, nullptr, nullptr, dH);
+}
 
 int rz_simt_forward(const RzLaunchCtx &c, const void *X, const float *hashed, const float *bias, void *Y)
 {

@@ -1,0 +1,235 @@
+// Tensor-core launches of products grouped by row: block shapes and descriptors for the GROUPED instantiations of
+// rz_tc_kernel.cuh.  The number of blocks is known on the device only, so every launch fills the machine (one CTA or CTA pair per
+// SM or pair of SMs) and the kernel deals the planned pieces' blocks out round robin.
+#include <atomic>
+#include <cstring>
+
+#include "rz_tc_host.h"
+#include "rz_tc_kernel.cuh"
+
+using namespace rztc;
+
+namespace {
+
+int usable_sms(const rz_problem *pb)
+{
+    const int n = num_sms() - (pb->sm_reserve > 0 ? pb->sm_reserve : 0);
+    return n < 2 ? 2 : n;
+}
+
+template <int OP, bool TF32, int CTAS, int RB, int SPLIT, int NC, int EW = 1>
+int launch(const RzLaunchCtx &c, const CUtensorMap &mapA, const CUtensorMap &mapB, const CUtensorMap &mapC, TcGroupParams &p,
+           const RzGroupPieces &pieces)
+{
+    const rz_problem *pb = c.pb;
+    constexpr int ES = TF32 ? 4 : 2, KC = 128 / ES, PAIR_R = TILE_R * CTAS, ITEM_R = PAIR_R * RB;
+    constexpr int SMEM_TOTAL = smem_total(OP, CTAS, RB, SPLIT, NC, EW);
+    static_assert(SMEM_TOTAL <= SMEM_LIMIT, "shared memory budget");
+    p.hash = c.hash;
+    p.M = (uint32_t)pb->M, p.K = (uint32_t)pb->K, p.N = (uint32_t)pb->N;
+    p.rows = OP == OP_DW ? p.N : p.M;   // (the weight gradient is computed transposed: N x K)
+    p.cols = OP == OP_FWD ? p.N : p.K;
+    p.tiles_r = OP == OP_DW ? (p.rows + ITEM_R - 1) / ITEM_R : 0;   // FWD, DX: the planned pieces
+    p.tiles_c = (p.cols + NC - 1) / NC;
+    p.nchunks = ((OP == OP_FWD ? p.K : p.N) + KC - 1) / KC;         // DW: a piece's rows
+    const uint32_t stage = (uint32_t)KC, bk = (uint32_t)pb->BK, bcols = (uint32_t)(NC / CTAS);
+    p.br = OP == OP_FWD ? (bk < stage ? bk : stage) : (bk < bcols ? bk : bcols);
+    p.kparts = stage / (bk < stage ? bk : stage);
+    p.group_rows = GROUP_ROWS / RB;
+    p.nsplit = 1, p.chunks_per_split = p.nchunks;
+    p.n_main = 0xffffffffu;   // every block runs its whole contraction
+    p.total_items = 0, p.units = 0;
+    p.alpha = pb->alpha;
+    p.relu = (pb->flags & RZ_FLAG_RELU) ? 1 : 0;
+    p.tma_store = 1;
+    p.header = pieces.header, p.entries = pieces.entries, p.group_tiles = pieces.group_tiles;
+    int st = rz_wait_context(&p.wait, 2000000000ll);   // also refuses to launch behind a kernel whose wait gave up
+    if (st) return st;
+
+    // shared-memory descriptors (bytes), as in the ungrouped launches
+    const uint32_t atom = KC * 128, mn_kstep = (TF32 ? 8 : 16) * 128, mn_sbo = TF32 ? 512 : 1024, mn_layout = TF32 ? 1 : 2;
+    p.a_layout = p.b_layout = 2;
+    p.a_lbo = p.b_lbo = 16, p.a_sbo = p.b_sbo = 1024, p.a_kstep = p.b_kstep = 32;   // K-major
+    if (OP != OP_DX) p.b_lbo = atom, p.b_sbo = mn_sbo, p.b_kstep = mn_kstep, p.b_layout = mn_layout;
+    if (OP == OP_DW) p.a_lbo = atom, p.a_sbo = mn_sbo, p.a_kstep = mn_kstep, p.a_layout = mn_layout;
+    const uint32_t a_major = OP == OP_DW ? 1u : 0u, b_major = OP == OP_DX ? 0u : 1u, fmt = TF32 ? 2u : 1u;
+    p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a_major << 15) | (b_major << 16) | ((uint32_t)(NC >> 3) << 17) |
+              ((uint32_t)(PAIR_R >> 4) << 24);
+
+    auto kern = rz_tc_kernel<OP, TF32, CTAS, RB, SPLIT, NC, EW, 1>;
+    // per kernel variant and device, once: the shared-memory opt-in and how many clusters fit the device
+    static std::atomic<int> ready[64];   // 0 = not set up, else resident blocks / pairs + 1
+    int dev = 0;
+    st = rz_record_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+    if (st) return st;
+    const bool cacheable = dev >= 0 && dev < 64;
+    const int known = cacheable ? ready[dev].load(std::memory_order_acquire) : 0;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attr[1];
+    cfg.blockDim = dim3(num_threads(RB, SPLIT, EW), 1, 1);
+    cfg.dynamicSmemBytes = SMEM_TOTAL;
+    cfg.stream = c.stream;
+    int slots = num_sms() / CTAS;
+    if (CTAS == 2) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cfg.gridDim = dim3(2 * (unsigned)slots, 1, 1);
+    }
+    if (known) {
+        slots = known - 1;
+    } else {
+        st = rz_record_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL),
+                            "set max dynamic shared memory");
+        if (st) return st;
+        if (CTAS == 2) {
+            int clusters = 0;
+            if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0 && clusters < slots)
+                slots = clusters;
+            (void)cudaGetLastError();
+        }
+        if (cacheable) ready[dev].store(slots + 1, std::memory_order_release);
+    }
+    if (pb->sm_reserve > 0) {
+        slots -= (pb->sm_reserve + CTAS - 1) / CTAS;
+        if (slots < 1) slots = 1;
+    }
+    const uint64_t most = (uint64_t)pieces.most * p.tiles_c * (OP == OP_DW ? p.tiles_r : 1);
+    if (most >= 0x80000000ull) return RZ_ERR_SHAPE;   // block numbers are 32-bit words
+    cfg.gridDim = dim3((unsigned)(most < (uint64_t)slots ? most : (uint64_t)slots) * CTAS, 1, 1);
+    st = rz_record_cuda(cudaLaunchKernelEx(&cfg, kern, mapA, mapB, mapC, p), "grouped tcgen05 kernel launch");
+    rz_count_launch(1);
+    if (st) return st;
+    return rz_record_cuda(cudaGetLastError(), "grouped tcgen05 kernel launch");
+}
+
+template <int OP>
+int launch_any(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const CUtensorMap &mapA, const CUtensorMap &mapB, const CUtensorMap &mapC,
+               TcGroupParams &p, const RzGroupPieces &pieces)
+{
+    const bool tf32 = c.pb->precision == RZ_PREC_TF32;
+    if (c.pb->precision == RZ_PREC_FP32) {
+        if (plan.nc == 128) return launch<OP, true, 1, 1, 1, 128>(c, mapA, mapB, mapC, p, pieces);
+        return launch<OP, true, 1, 1, 1, 64>(c, mapA, mapB, mapC, p, pieces);
+    }
+    constexpr int W1 = OP == OP_DW ? 4 : 1, W2 = OP == OP_DW ? 2 : 1;   // epilogue warps per TMEM lane quarter and row block
+    if (plan.rb == 2)
+        return tf32 ? launch<OP, true, 2, 2, 0, 256, W2>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 2, 2, 0, 256, W2>(c, mapA, mapB, mapC, p, pieces);
+    if (plan.ctas == 2)
+        return tf32 ? launch<OP, true, 2, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 2, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces);
+    if (plan.nc == 256)
+        return tf32 ? launch<OP, true, 1, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 1, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces);
+    if (plan.nc == 128)
+        return tf32 ? launch<OP, true, 1, 1, 0, 128, W1>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 1, 1, 0, 128, W1>(c, mapA, mapB, mapC, p, pieces);
+    return tf32 ? launch<OP, true, 1, 1, 0, 64, W1>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 1, 1, 0, 64, W1>(c, mapA, mapB, mapC, p, pieces);
+}
+
+}  // namespace
+
+// Block shape by an estimate of the time: waves of blocks over the SMs, times a block's stages (or, weight gradient, its
+// scatter where that is longer), at the relative tensor throughput each shape sustains.  The host knows the rows and the groups
+// but not how the rows are spread: it reckons with even groups, each with half a ragged block at its end.
+RzTcGroupPlan rz_tc_grouped_plan(const rz_problem *pb, int groups, int op)
+{
+    static const struct {
+        int ctas, rb, nc;
+        double speed;
+    } shapes[] = {{2, 2, 256, 1.00}, {2, 1, 256, 0.80}, {1, 1, 256, 0.58}, {1, 1, 128, 0.40}, {1, 1, 64, 0.25}};
+    const bool bf16 = pb->precision == RZ_PREC_BF16, split = pb->precision == RZ_PREC_FP32, dw = op == RZ_OP_BACKWARD_WEIGHT;
+    const double kc = bf16 ? 64.0 : 32.0;
+    const double used = (double)(pb->M < groups ? pb->M : groups), mean = (double)pb->M / used;
+    const int64_t cols = op == RZ_OP_FORWARD ? pb->N : pb->K;
+    const int sms = usable_sms(pb);
+    RzTcGroupPlan best = {1, 1, 64, 4, 128};
+    double best_time = -1.0;
+    const int forced = forced_shape();
+    for (int i = 0; i < 5; ++i) {
+        const auto &s = shapes[i];
+        // split precision: no pairs, and at least three chains; seven where three would be longer than 1440 elements (4e-6)
+        const int64_t depth = dw ? 2048 : op == RZ_OP_FORWARD ? pb->K : pb->N;
+        if (split && (s.ctas == 2 || s.nc == 256 || (s.nc == 128 && depth > 3 * 1440))) continue;
+        const int64_t bcols = s.nc / s.ctas;                   // whole B boxes per hash tile (input gradient)
+        if (op == RZ_OP_BACKWARD_INPUT && (pb->BK <= bcols ? bcols % pb->BK != 0 : pb->BK % bcols != 0)) continue;
+        const double slots = (double)(sms / s.ctas), tiles_c = (double)((cols + s.nc - 1) / s.nc);
+        const int item_r = TILE_R * s.ctas * s.rb;
+        double items, stages;
+        uint32_t step = (uint32_t)item_r;
+        if (dw) {
+            // at most 2048 rows in one accumulation chain: the tensor core truncates when it adds
+            step = 2048;
+            const double blocks = (double)((pb->N + item_r - 1) / item_r) * tiles_c;
+            const double pieces = used * (double)((int64_t)((mean + step - 1) / step));
+            items = pieces * blocks;
+            stages = mean * used / pieces / kc + 1.0;
+            if (s.rb == 2) stages += 19.0;                     // its scatter does not overlap the next block
+            else if (stages < 8.0) stages = 8.0;               // shorter contractions are bound by the scatter
+        } else {
+            const double per_group = mean / item_r + 0.5;
+            items = used * (per_group < 1.0 ? 1.0 : per_group) * tiles_c;
+            stages = (double)((op == RZ_OP_FORWARD ? pb->K : pb->N)) / kc + (s.rb == 2 ? 10.0 : 3.0);
+        }
+        double waves = items / slots;
+        waves = waves < 1.0 ? 1.0 : waves + 0.5;               // half a wave is lost at the end
+        const double time = waves * stages * (double)(s.rb * s.nc) / s.speed;
+        if (best_time < 0.0 || time < best_time || i == forced) {
+            best_time = i == forced ? 0.0 : time;
+            best.ctas = s.ctas, best.rb = s.rb, best.nc = s.nc, best.ew = dw && !split ? (s.rb == 2 ? 2 : 4) : 1, best.step = step;
+        }
+    }
+    return best;
+}
+
+int rz_tc_grouped_forward(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *X, const void *copies,
+                          const float *bias, void *Y)
+{
+    const rz_problem *pb = c.pb;
+    const bool tf32 = pb->precision != RZ_PREC_BF16;
+    const Geometry g = geometry(pb);
+    TcGroupParams p;
+    memset(&p, 0, sizeof(p));
+    p.bias = bias;
+    p.out = Y;
+    CUtensorMap mapA, mapB, mapC;
+    int st = map_matrix(&mapA, tf32, false, X, pb->M, pb->K, g.epr, TILE_R);
+    if (st) return st;
+    st = map_shadow(&mapB, pb, true, copies, pb->BK < g.epr ? pb->BK : g.epr);
+    if (st) return st;
+    st = map_matrix(&mapC, tf32, false, Y, pb->M, pb->N, g.epr, 32);
+    if (st) return st;
+    return launch_any<OP_FWD>(c, plan, mapA, mapB, mapC, p, pieces);
+}
+
+int rz_tc_grouped_backward_input(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *dY,
+                                 const void *copies, void *dX)
+{
+    const rz_problem *pb = c.pb;
+    const bool tf32 = pb->precision != RZ_PREC_BF16;
+    const Geometry g = geometry(pb);
+    TcGroupParams p;
+    memset(&p, 0, sizeof(p));
+    p.out = dX;
+    CUtensorMap mapA, mapB, mapC;
+    int st = map_matrix(&mapA, tf32, false, dY, pb->M, pb->N, g.epr, TILE_R);
+    if (st) return st;
+    const uint32_t bcols = (uint32_t)(plan.nc / plan.ctas);
+    st = map_shadow(&mapB, pb, false, copies, (uint32_t)pb->BK < bcols ? (uint32_t)pb->BK : bcols);
+    if (st) return st;
+    st = map_matrix(&mapC, tf32, false, dX, pb->M, pb->K, g.epr, 32);
+    if (st) return st;
+    return launch_any<OP_DX>(c, plan, mapA, mapB, mapC, p, pieces);
+}
+
+int rz_tc_grouped_backward_weight(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *maps, float *dH)
+{
+    TcGroupParams p;
+    memset(&p, 0, sizeof(p));
+    p.dH = dH;
+    p.maps = static_cast<const CUtensorMap *>(maps);
+    CUtensorMap unused;   // the groups' own maps are on the device
+    memset(&unused, 0, sizeof(unused));
+    return launch_any<OP_DW>(c, plan, unused, unused, unused, p, pieces);
+}

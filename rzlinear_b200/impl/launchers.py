@@ -65,7 +65,7 @@ def alloc_shadow(pb, hashed: torch.Tensor) -> Optional[torch.Tensor]:
 _CACHE_ATTR = "_rz_shadow_cache"
 
 
-def cached_shadow(pb, hashed_weight: torch.Tensor, hashed_f32: torch.Tensor) -> Optional[torch.Tensor]:
+def cached_shadow(pb, hashed_weight: torch.Tensor, hashed_f32: torch.Tensor, nbytes: Optional[int] = None) -> Optional[torch.Tensor]:
     """The shadow of `hashed_weight` for this problem, rebuilt only when the weights have changed.
 
     The cache lives on the tensor object itself (so it dies with it and can never be mistaken for another
@@ -77,9 +77,12 @@ def cached_shadow(pb, hashed_weight: torch.Tensor, hashed_f32: torch.Tensor) -> 
     micro-batches per optimiser step) therefore allocates nothing and launches no refresh.
     While a CUDA graph is being captured the refresh is always launched (it becomes a node of the graph): a replay
     runs none of this Python, so a graph that skipped the refresh would keep reading the shadow of the weights it
-    was captured with."""
+    was captured with.
+    `nbytes`: what the buffer has to hold (default: what the linear layer's calls need, their workspace included; grouped
+    calls need the shifted copies alone)."""
     _lib._require_cuda(hashed_f32)
-    nbytes = _lib.shadow_bytes(pb)
+    if nbytes is None:
+        nbytes = _lib.shadow_bytes(pb)
     if nbytes == 0:
         return None
     cache = getattr(hashed_weight, _CACHE_ATTR, None)

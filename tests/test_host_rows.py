@@ -88,3 +88,52 @@ def test_embedding_draws_the_linear_layers_numbers_without_reseeding():
     assert torch.equal(torch.rand(3), want)
     assert torch.equal(emb._random_numbers, rz.RzLinear(64, 64, seed=31)._random_numbers)
     assert emb._random_numbers.dtype == torch.int32
+
+
+def test_grouped_refusals(rzlib):
+    lib = rzlib.load()
+    some, odd = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8)
+    ref = ctypes.byref
+    pb = _pb(rzlib, M=100, K=128, N=192, H=8192, BK=32, BN=64, io=1, prec=2)
+    assert rzlib.plan(pb, 0) == rzlib.PATH_TCGEN05
+    copies, ws = lib.rz_grouped_copies_bytes(ref(pb)), lib.rz_grouped_workspace_bytes(ref(pb), 4)
+    assert copies == 8 * 8192 * 2 and ws > 0 and ws % 256 == 0
+    assert lib.rz_grouped_copies_bytes(ref(_pb(rzlib, BK=16))) == 0
+
+    def fwd(pb=pb, groups=4, off=some, x=some, h=some, c=some, cb=copies, y=some, w=some, wb=ws):
+        return lib.rz_grouped_forward(ref(pb), groups, off, x, h, c, cb, None, y, w, wb, None)
+
+    assert fwd(groups=0) == -2 and fwd(groups=-1) == -2 and fwd(groups=4097) == -10
+    assert fwd(pb=_pb(rzlib, K=1 << 20, BK=32, BN=64), groups=2048) == -2              # stacked rows pass 2^31
+    assert fwd(off=None) == -1 and fwd(x=None) == -1 and fwd(y=None) == -1 and fwd(c=None) == -1 and fwd(w=None) == -1
+    assert fwd(cb=copies - 1) == -11 and fwd(wb=ws - 1) == -11
+    assert fwd(x=odd) == -5 and fwd(y=odd) == -5 and fwd(w=odd) == -5 and fwd(off=ctypes.c_void_p((1 << 20) + 2)) == -5
+    assert lib.rz_grouped_backward_weight(ref(pb), 4, some, some, some, None, some, ws, None) == -1
+    assert lib.rz_grouped_backward_weight(ref(pb), 4, some, some, some, some, some, ws - 1, None) == -11
+    assert lib.rz_grouped_backward_input(ref(pb), 4, some, None, some, some, copies, some, some, ws, None) == -1
+    assert lib.rz_grouped_grad_prepare(ref(pb), 4, some, some, None, None, None, some, ws, None) == -1
+    assert lib.rz_grouped_grad_prepare(ref(pb), 4, some, some, some, None, some, some, ws, None) == -1   # a mask, nowhere to write
+
+    layer = rz.RzGroupedLinear(4, 128, 64)
+    assert layer._hashed_weight.shape == (2048,) and layer._bias.shape == (4, 64)
+    off, x = torch.zeros(5, dtype=torch.int32), torch.randn(6, 128)
+    with pytest.raises(AssertionError):
+        layer(x, off)                                                                   # H = 2048 <= 32 * 64
+    layer = rz.RzGroupedLinear(4, 128, 64, compress_ratio=0.5)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        layer(x, off)
+    with pytest.raises(ValueError):
+        layer(x, off[:4])
+    with pytest.raises(ValueError):
+        layer(x[None], off)
+    with pytest.raises(ValueError):
+        layer(x[:, :64], off)
+    with pytest.raises(TypeError):
+        layer(x, off.float())
+    with pytest.raises(TypeError):
+        layer(x.int(), off)
+    for bad in (0, 4097):
+        with pytest.raises(ValueError):
+            rz.RzGroupedLinear(bad, 128, 64)
+    with pytest.raises(ValueError):
+        rz.RzGroupedLinearFunction.apply(x, layer._hashed_weight, layer._random_numbers, off, 64, 1.0, None, torch.zeros(64))
