@@ -195,18 +195,20 @@ int rz_sort_rows(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order
 
 /* Embedding lookup in a virtual table W[K,N] of K rows: out[M,N] (io_dtype) = alpha * W[ids[m], :], read from the fp32
    hashed array itself.  A token whose id is outside [0, K) or equal to padding_idx gives a row of zeros (pass a negative
-   padding_idx for none).  `precision` must go with io_dtype and is otherwise unused. */
+   padding_idx for none).  `precision` must go with io_dtype and is otherwise unused.
+   `plan` (4-byte aligned, rz_embedding_plan_bytes() bytes; NULL when no gradient will be asked for) receives the tokens sorted in
+   chunks, which the gradient wants; the sort runs beside the lookup. */
+size_t rz_embedding_plan_bytes(const rz_problem *pb);
 int rz_embedding_forward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const float *hashed, void *out,
-                         void *stream);
+                         void *plan, size_t plan_bytes, void *stream);
 
 /* Its gradient: dH[offset(k / BK, n / BN) + (k % BK) * BN + n % BN] += alpha * (sum of dOut[m, n] over the tokens with
    ids[m] = k), fp32; dH is zeroed first unless RZ_FLAG_ACCUMULATE_DH.  Tokens that gave zeros contribute nothing, whatever
-   their dOut holds.  Tokens are sorted in chunks, and the rows of one token summed, before anything is added into dH; those additions
-   are fp32 reductions whose order is not fixed, as in rz_linear_backward_weight.  `scratch` (4-byte aligned):
-   rz_embedding_scratch_bytes() bytes during the call (0 for short batches; then it may be NULL). */
-size_t rz_embedding_scratch_bytes(const rz_problem *pb);
+   their dOut holds.  With the plan that rz_embedding_forward made of the same ids, K and padding_idx, the rows of equal tokens are
+   summed before they are added into dH; without one (NULL) every token's row is added by itself, which is right and, where tokens
+   repeat, slow.  The additions are fp32 reductions whose order is not fixed, as in rz_linear_backward_weight. */
 int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const void *dOut, float *dH,
-                          void *scratch, size_t scratch_bytes, void *stream);
+                          const void *plan, size_t plan_bytes, void *stream);
 
 /* ---- products grouped by row (the experts of a layer) -----------------------------------------
    M rows in `groups` consecutive groups: rows offsets[g] .. offsets[g + 1) belong to group g (int32 [groups + 1], on the device; the
@@ -229,20 +231,17 @@ int rz_grouped_forward(const rz_problem *pb, int64_t groups, const int32_t *offs
                        const void *copies, size_t copies_bytes, const float *bias, void *Y, void *workspace, size_t workspace_bytes,
                        void *stream);
 
-/* dX[r,:] = alpha * dY[r,:] . W_g^T. */
-int rz_grouped_backward_input(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *dY, const float *hashed,
-                              const void *copies, size_t copies_bytes, void *dX, void *workspace, size_t workspace_bytes,
-                              void *stream);
-
-/* dH[word of W_g[k,n]] += alpha * sum over the rows r of group g of X[r,k] dY[r,n], for every group; dH is zeroed first unless
-   RZ_FLAG_ACCUMULATE_DH. */
-int rz_grouped_backward_weight(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const void *dY, float *dH,
-                               void *workspace, size_t workspace_bytes, void *stream);
-
-/* rz_grad_prepare with a bias for each group: bias_grad fp32 [groups, N].  Rows of dYm that belong to no group are not written
-   (the grouped calls do not look at them). */
-int rz_grouped_grad_prepare(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *dY, const void *Y, void *dYm,
-                            float *bias_grad, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients of rz_grouped_forward, any of them (NULL for the ones not wanted):
+     dX[r,:] = alpha * dY[r,:] . W_g^T;
+     dH[word of W_g[k,n]] += alpha * sum over the rows r of group g of X[r,k] dY[r,n], for every group, zeroed first unless
+       RZ_FLAG_ACCUMULATE_DH (fp32 reductions whose order is not fixed, as in rz_linear_backward_weight);
+     bias_grad[g,:] = sum over the rows of group g of dY[r,:], fp32 [groups, N], zeroed first (fp32 reductions too).
+   For a layer with a ReLU, Y is its saved output and dY counts only where Y > 0; dYm [M,N] receives the masked gradient (its rows of
+   no group are not written).  X may be NULL when dH is, hashed and copies when dX is.  rz_plan()'s TCGEN05 path wants X, dY, dYm
+   and dX 16-byte aligned. */
+int rz_grouped_backward(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const void *dY, const void *Y,
+                        const float *hashed, const void *copies, size_t copies_bytes, void *dYm, float *bias_grad, void *dX, float *dH,
+                        void *workspace, size_t workspace_bytes, void *stream);
 
 /* Number of kernels this library has launched in this process (all threads). */
 uint64_t rz_launch_count(void);

@@ -7,7 +7,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .RzLinearFunction import DEFAULT_CONFIG, RzConfig, _compute_view, _unpack, controls
+from .RzLinearFunction import DEFAULT_CONFIG, RzConfig, _compute_view, controls
 from .impl import launchers
 
 
@@ -22,7 +22,50 @@ def _offsets_view(offsets: torch.Tensor, rows: int) -> torch.Tensor:
     return offsets.detach().contiguous()
 
 
+def _as(t, dtype, shape=None):
+    """t in another dtype and shape, where it has others (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if shape is None or t.shape == shape else t.view(shape)
+
+
+def _product(input, hashed_weight, random_numbers, offsets, output_dim, init_factor, config, bias):
+    """(output in the compute dtype, int32 offsets, problem, groups, shifted copies): the forward pass and what the backward wants of it."""
+    cfg = config if config is not None else DEFAULT_CONFIG
+    if input.dim() != 2:
+        raise ValueError(f"RzGroupedLinear takes (rows, input_dim) activations, got {input.dim()} dimensions")
+    M, K, N, H = input.shape[0], input.shape[1], output_dim, hashed_weight.numel()
+    off = _offsets_view(offsets, M)
+    groups = off.numel() - 1
+    if bias is not None and tuple(bias.shape) != (groups, N):
+        raise ValueError(f"bias must have shape {(groups, N)}, got {tuple(bias.shape)}")
+    x = _compute_view(input)
+    hashed = launchers._hashed_f32(hashed_weight)
+    pb = launchers.cached_problem(max(1, M), K, N, H, random_numbers, cfg.block_size_k, cfg.block_size_n, x.dtype,
+                                  controls['triton_allow_tf32'], init_factor, cfg.hash_mode, _lib.FLAG_RELU if cfg.relu else 0)
+    _lib._require_together(x, hashed, off, bias)
+    copies_bytes, ws_bytes = _lib.grouped_sizes(pb, groups)
+    copies = launchers.cached_shadow(pb, hashed_weight, hashed, copies_bytes) if M else None
+    out = torch.empty((M, N), device=x.device, dtype=x.dtype)
+    b = None if bias is None else bias.detach().float().contiguous()
+    if M:
+        _lib.grouped_forward(pb, groups, off, x, hashed, copies, b, out,
+                             torch.empty(ws_bytes, dtype=torch.uint8, device=x.device))
+    return out, off, pb, groups, copies
+
+
 class RzGroupedLinearFunction(torch.autograd.Function):
+    @classmethod
+    def apply(cls, *args):
+        # nothing to differentiate: the product alone, without the autograd machinery
+        if not (torch.is_grad_enabled() and any(a.requires_grad for a in (args[0], args[1], *args[7:]) if a is not None)):
+            with torch.no_grad():
+                out = _product(*args, *(None,) * (8 - len(args)))[0]
+                return out if out.dtype == args[0].dtype else out.to(args[0].dtype)
+        return super().apply(*args, *(None,) * (8 - len(args)))
+
     @staticmethod
     def forward(ctx, input: torch.Tensor, hashed_weight: torch.Tensor, random_numbers: torch.Tensor, offsets: torch.Tensor,
                 output_dim, init_factor, config: Optional[RzConfig] = None, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -41,28 +84,11 @@ class RzGroupedLinearFunction(torch.autograd.Function):
                 output (Tensor): (M, output_dim).  Rows that belong to no group (before offsets[0], behind the last offset) are
                 zeros and get no gradient.
         '''
-        cfg = config if config is not None else DEFAULT_CONFIG
-        if input.dim() != 2:
-            raise ValueError(f"RzGroupedLinear takes (rows, input_dim) activations, got {input.dim()} dimensions")
-        M, K, N, H = input.shape[0], input.shape[1], output_dim, hashed_weight.numel()
-        off = _offsets_view(offsets, M)
-        groups = off.numel() - 1
-        if bias is not None and tuple(bias.shape) != (groups, N):
-            raise ValueError(f"bias must have shape {(groups, N)}, got {tuple(bias.shape)}")
-        x = _compute_view(input)
-        hashed = launchers._hashed_f32(hashed_weight)
-        pb = launchers.make_problem(max(1, M), K, N, H, _unpack(random_numbers), cfg.block_size_k, cfg.block_size_n, x.dtype,
-                                    controls['triton_allow_tf32'], init_factor, cfg.hash_mode, _lib.FLAG_RELU if cfg.relu else 0)
-        _lib._require_together(x, hashed, off, bias)
-        copies = launchers.cached_shadow(pb, hashed_weight, hashed, _lib.grouped_copies_bytes(pb)) if M else None
-        out = torch.empty((M, N), device=x.device, dtype=x.dtype)
-        b = None if bias is None else bias.detach().float().contiguous()
-        if M:
-            _lib.grouped_forward(pb, groups, off, x, hashed, copies, b, out, _lib.grouped_workspace(pb, groups, x.device))
-
+        out, off, pb, groups, copies = _product(input, hashed_weight, random_numbers, offsets, output_dim, init_factor, config, bias)
         # (the saved output keeps the compute dtype: the backward masks with it)
-        ctx.save_for_backward(input, hashed_weight, off, out if cfg.relu else None)
-        ctx.pb, ctx.groups, ctx.relu = pb, groups, cfg.relu
+        relu = bool(pb.flags & _lib.FLAG_RELU)
+        ctx.save_for_backward(input, hashed_weight, off, out if relu else None)
+        ctx.pb, ctx.groups, ctx.relu = pb, groups, relu
         ctx.copies = copies  # the backward reads the weights the forward saw
         ctx.bias_dtype = None if bias is None else bias.dtype
         return out if out.dtype == input.dtype else out.to(input.dtype)
@@ -71,33 +97,17 @@ class RzGroupedLinearFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         input, hashed_weight, off, out = ctx.saved_tensors
-        pb, groups = _lib.with_fields(ctx.pb, flags=0), ctx.groups
-        M, K, N = input.shape[0], pb.K, pb.N
-        input_grad = weight_grad = bias_grad = None
+        pb, groups = ctx.pb, ctx.groups
         x = _compute_view(input)
-        grad = grad.to(x.dtype).contiguous()
-        ws = _lib.grouped_workspace(pb, groups, x.device)
-        # one pass over the incoming gradient: ReLU mask from the saved output and the bias gradients (column sums)
-        want_bias = ctx.bias_dtype is not None and ctx.needs_input_grad[7]
-        if ctx.relu or want_bias:
-            masked = torch.empty_like(grad) if ctx.relu else None
-            bias_grad = (torch.empty if M else torch.zeros)((groups, N), device=x.device, dtype=torch.float32) if want_bias else None
-            if M:
-                _lib.grouped_grad_prepare(pb, groups, off, grad, out if ctx.relu else None, masked, bias_grad, ws)
-            if ctx.relu:
-                grad = masked
-            if want_bias:
-                bias_grad = bias_grad.to(ctx.bias_dtype)
-        if ctx.needs_input_grad[0]:
-            input_grad = torch.empty((M, K), device=x.device, dtype=x.dtype)
-            if M:
-                _lib.grouped_backward_input(pb, groups, off, grad, launchers._hashed_f32(hashed_weight), ctx.copies, input_grad, ws)
-            input_grad = input_grad.to(input.dtype)
-        if ctx.needs_input_grad[1]:
-            dh = torch.empty((pb.H,), device=x.device, dtype=torch.float32)
-            if M:
-                _lib.grouped_backward_weight(pb, groups, off, x, grad, dh, ws)   # zeroes dh first
-            else:
-                dh.zero_()
-            weight_grad = dh.to(hashed_weight.dtype).view(hashed_weight.shape)
-        return input_grad, weight_grad, None, None, None, None, None, bias_grad
+        M, make = input.shape[0], torch.empty if input.shape[0] else torch.zeros
+        grad = _as(grad, x.dtype).contiguous()
+        dx = make((M, pb.K), device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
+        dh = make((pb.H,), device=x.device, dtype=torch.float32) if ctx.needs_input_grad[1] else None
+        bias_grad = make((groups, pb.N), device=x.device, dtype=torch.float32) if ctx.needs_input_grad[7] else None
+        if M:
+            hashed = None if dx is None else launchers._hashed_f32(hashed_weight)
+            _lib.grouped_backward(pb, groups, off, x, grad, out if ctx.relu else None, hashed, ctx.copies,
+                                  torch.empty_like(grad) if ctx.relu else None, bias_grad, dx, dh,
+                                  torch.empty(_lib.grouped_sizes(pb, groups)[1], dtype=torch.uint8, device=x.device))
+        return (_as(dx, input.dtype), _as(dh, hashed_weight.dtype, hashed_weight.shape), None, None, None, None, None,
+                _as(bias_grad, ctx.bias_dtype))

@@ -31,8 +31,8 @@ EXPORTS = [
     "rz_linear_materialize", "rz_sgd_step", "rz_device_status", "rz_launch_count",
     "rz_selftest_bounded_wait", "rz_sgd_momentum_step", "rz_grad_prepare", "rz_linear_forward_noalloc",
     "rz_reload_env", "rz_sort_rows", "rz_sort_rows_scratch_bytes", "rz_embedding_forward",
-    "rz_embedding_scratch_bytes", "rz_embedding_backward", "rz_grouped_copies_bytes", "rz_grouped_workspace_bytes",
-    "rz_grouped_forward", "rz_grouped_backward_input", "rz_grouped_backward_weight", "rz_grouped_grad_prepare",
+    "rz_embedding_plan_bytes", "rz_embedding_backward", "rz_grouped_copies_bytes", "rz_grouped_workspace_bytes",
+    "rz_grouped_forward", "rz_grouped_backward",
 ]
 
 
@@ -97,26 +97,23 @@ def load() -> ctypes.CDLL:
         lib.rz_sort_rows_scratch_bytes.argtypes = [i64, i64]
         lib.rz_sort_rows_scratch_bytes.restype = sz
         lib.rz_sort_rows.argtypes = [vp, i64, i64, vp, vp, vp, sz, vp]
-        lib.rz_embedding_forward.argtypes = [pbp, vp, i64, vp, vp, vp]
-        lib.rz_embedding_scratch_bytes.argtypes = [pbp]
-        lib.rz_embedding_scratch_bytes.restype = sz
+        lib.rz_embedding_forward.argtypes = [pbp, vp, i64, vp, vp, vp, sz, vp]
+        lib.rz_embedding_plan_bytes.argtypes = [pbp]
+        lib.rz_embedding_plan_bytes.restype = sz
         lib.rz_embedding_backward.argtypes = [pbp, vp, i64, vp, vp, vp, sz, vp]
         lib.rz_grouped_copies_bytes.argtypes = [pbp]
         lib.rz_grouped_copies_bytes.restype = sz
         lib.rz_grouped_workspace_bytes.argtypes = [pbp, i64]
         lib.rz_grouped_workspace_bytes.restype = sz
         lib.rz_grouped_forward.argtypes = [pbp, i64, vp, vp, vp, vp, sz, vp, vp, vp, sz, vp]
-        lib.rz_grouped_backward_input.argtypes = [pbp, i64, vp, vp, vp, vp, sz, vp, vp, sz, vp]
-        lib.rz_grouped_backward_weight.argtypes = [pbp, i64, vp, vp, vp, vp, vp, sz, vp]
-        lib.rz_grouped_grad_prepare.argtypes = [pbp, i64, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.rz_grouped_backward.argtypes = [pbp, i64, vp, vp, vp, vp, vp, vp, sz, vp, vp, vp, vp, vp, sz, vp]
         lib.rz_device_status.argtypes = [ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]
         lib.rz_launch_count.restype = ctypes.c_uint64
         for name in ("rz_hash_indices_host", "rz_hash_indices_device", "rz_plan", "rz_shadow_refresh",
                      "rz_linear_forward", "rz_linear_backward_input", "rz_linear_backward_weight",
                      "rz_linear_materialize", "rz_sgd_step", "rz_device_status", "rz_sgd_momentum_step",
                      "rz_selftest_bounded_wait", "rz_linear_forward_noalloc", "rz_sort_rows", "rz_embedding_forward",
-                     "rz_embedding_backward", "rz_grouped_forward", "rz_grouped_backward_input", "rz_grouped_backward_weight",
-                     "rz_grouped_grad_prepare"):
+                     "rz_embedding_backward", "rz_grouped_forward", "rz_grouped_backward"):
             getattr(lib, name).restype = ctypes.c_int
         _lib = lib
     return _lib
@@ -187,11 +184,12 @@ class _on:
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()      # (the argtypes make a void * of the integer)
 
 
-def _stream(device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _stream(device) -> int:
+    """cudaStream_t of the current stream, without building a torch.cuda.Stream: small problems are bound by host time."""
+    return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
 
 
 def _require_cuda(*tensors):
@@ -202,10 +200,17 @@ def _require_cuda(*tensors):
 
 def _require_together(*tensors):
     """CUDA tensors, all on one device."""
-    _require_cuda(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise RuntimeError(f"rzlinear_b200: tensors of one call must be on one device, got {sorted(map(str, devices))}")
+    index = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _require_cuda(t)
+        at = t.get_device()
+        if index is None:
+            index = at
+        elif at != index:
+            raise RuntimeError(f"rzlinear_b200: tensors of one call must be on one device, got cuda:{index} and cuda:{at}")
 
 
 def _scratch(nbytes: int, device):
@@ -297,28 +302,34 @@ def sort_rows(keys, bins, order, offsets) -> None:
                                   _stream(keys.device)))
 
 
-def embedding_forward(pb, ids, padding_idx, hashed, out) -> None:
-    _require_together(ids, hashed, out)
+def embedding_plan(pb, device):
+    """Buffer for the plan of an embedding's gradient (None for batches that need none)."""
+    return _scratch(int(load().rz_embedding_plan_bytes(ctypes.byref(pb))), device)
+
+
+def embedding_forward(pb, ids, padding_idx, hashed, out, plan=None) -> None:
+    _require_together(ids, hashed, out, plan)
     with _on(ids.device):
-        check(load().rz_embedding_forward(ctypes.byref(pb), _ptr(ids), padding_idx, _ptr(hashed), _ptr(out), _stream(ids.device)))
+        check(load().rz_embedding_forward(ctypes.byref(pb), _ptr(ids), padding_idx, _ptr(hashed), _ptr(out), _ptr(plan), _nbytes(plan),
+                                          _stream(ids.device)))
 
 
-def embedding_backward(pb, ids, padding_idx, dout, dh) -> None:
-    _require_together(ids, dout, dh)
-    scratch = _scratch(load().rz_embedding_scratch_bytes(ctypes.byref(pb)), ids.device)
+def embedding_backward(pb, ids, padding_idx, dout, dh, plan=None) -> None:
+    _require_together(ids, dout, dh, plan)
     with _on(ids.device):
-        check(load().rz_embedding_backward(ctypes.byref(pb), _ptr(ids), padding_idx, _ptr(dout), _ptr(dh), _ptr(scratch),
-                                           _nbytes(scratch), _stream(ids.device)))
+        check(load().rz_embedding_backward(ctypes.byref(pb), _ptr(ids), padding_idx, _ptr(dout), _ptr(dh), _ptr(plan), _nbytes(plan),
+                                           _stream(ids.device)))
 
 
-def grouped_copies_bytes(pb) -> int:
-    return int(load().rz_grouped_copies_bytes(ctypes.byref(pb)))
-
-
-def grouped_workspace(pb, groups: int, device):
-    """Workspace for the grouped calls of one stream; raises for a problem that rz_grouped_* would refuse."""
-    nbytes = int(load().rz_grouped_workspace_bytes(ctypes.byref(pb), groups))
-    return _scratch(max(nbytes, 256), device)
+def grouped_sizes(pb, groups: int):
+    """(bytes of shifted copies, bytes of workspace) of a grouped problem; remembered on the problem, which is never written to."""
+    known = getattr(pb, "_grouped_sizes", None)
+    if known is None or known[0] != groups:
+        lib = load()
+        known = (groups, int(lib.rz_grouped_copies_bytes(ctypes.byref(pb))),
+                 max(256, int(lib.rz_grouped_workspace_bytes(ctypes.byref(pb), groups))))
+        pb._grouped_sizes = known
+    return known[1:]
 
 
 def grouped_forward(pb, groups, offsets, x, hashed, copies, bias, y, ws) -> None:
@@ -328,26 +339,13 @@ def grouped_forward(pb, groups, offsets, x, hashed, copies, bias, y, ws) -> None
                                         _ptr(bias), _ptr(y), _ptr(ws), _nbytes(ws), _stream(x.device)))
 
 
-def grouped_backward_input(pb, groups, offsets, dy, hashed, copies, dx, ws) -> None:
-    _require_together(offsets, dy, hashed, copies, dx, ws)
+def grouped_backward(pb, groups, offsets, x, dy, y, hashed, copies, dym, bias_grad, dx, dh, ws) -> None:
+    """Gradients of grouped_forward; None for the ones not wanted.  With y (a ReLU's output) dym receives the masked gradient."""
+    _require_together(offsets, x, dy, y, hashed, copies, dym, bias_grad, dx, dh, ws)
     with _on(dy.device):
-        check(load().rz_grouped_backward_input(ctypes.byref(pb), groups, _ptr(offsets), _ptr(dy), _ptr(hashed), _ptr(copies),
-                                               _nbytes(copies), _ptr(dx), _ptr(ws), _nbytes(ws), _stream(dy.device)))
-
-
-def grouped_backward_weight(pb, groups, offsets, x, dy, dh, ws) -> None:
-    _require_together(offsets, x, dy, dh, ws)
-    with _on(x.device):
-        check(load().rz_grouped_backward_weight(ctypes.byref(pb), groups, _ptr(offsets), _ptr(x), _ptr(dy), _ptr(dh), _ptr(ws),
-                                                _nbytes(ws), _stream(x.device)))
-
-
-def grouped_grad_prepare(pb, groups, offsets, dy, y, dym, bias_grad, ws) -> None:
-    """dym = dy where y > 0 (y may be None), bias_grad[g] = column sums of group g's (masked) gradient (may be None)."""
-    _require_together(offsets, dy, y, dym, bias_grad, ws)
-    with _on(dy.device):
-        check(load().rz_grouped_grad_prepare(ctypes.byref(pb), groups, _ptr(offsets), _ptr(dy), _ptr(y), _ptr(dym), _ptr(bias_grad),
-                                             _ptr(ws), _nbytes(ws), _stream(dy.device)))
+        check(load().rz_grouped_backward(ctypes.byref(pb), groups, _ptr(offsets), _ptr(x), _ptr(dy), _ptr(y), _ptr(hashed), _ptr(copies),
+                                         _nbytes(copies), _ptr(dym), _ptr(bias_grad), _ptr(dx), _ptr(dh), _ptr(ws), _nbytes(ws),
+                                         _stream(dy.device)))
 
 
 def sgd_step(pb, hashed, dh, lr, shadow) -> None:

@@ -109,7 +109,7 @@ bool use_tc_grouped(const rz_problem *pb)
 
 // What the grouped entry points ask of their buffers besides that they exist.
 int check_grouped(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *in, const void *out, const void *copies,
-                  size_t copies_bytes, const void *workspace, size_t workspace_bytes, bool tc, bool needs_copies = true)
+                  size_t copies_bytes, const void *workspace, size_t workspace_bytes, bool tc, bool needs_copies)
 {
     if (!offsets || !workspace) return RZ_ERR_NULL;
     const uintptr_t element = pb->io_dtype == RZ_BF16 ? 2 : 4;
@@ -331,32 +331,33 @@ int rz_sort_rows(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order
     return rz_rows_sort(keys, rows, bins, order, offsets, scratch, reinterpret_cast<cudaStream_t>(stream));
 }
 
-int rz_embedding_forward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const float *hashed, void *out, void *stream)
+size_t rz_embedding_plan_bytes(const rz_problem *pb) { return validate(pb) ? 0 : rz_rows_embedding_plan(pb); }
+
+int rz_embedding_forward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const float *hashed, void *out, void *plan,
+                         size_t plan_bytes, void *stream)
 {
     int st = validate(pb);
     if (st) return st;
     if (!ids || !hashed || !out) return RZ_ERR_NULL;
-    if (!aligned_to(ids, 8) || !aligned_to(hashed, 4) || !aligned_to(out, pb->io_dtype == RZ_BF16 ? 2 : 4)) return RZ_ERR_ALIGN;
-    return rz_rows_embedding(make_ctx(pb, stream), ids, padding_idx, hashed, out);
+    if (plan && plan_bytes < rz_rows_embedding_plan(pb)) return RZ_ERR_SCRATCH;
+    if (!aligned_to(ids, 8) || !aligned_to(hashed, 4) || !aligned_to(out, pb->io_dtype == RZ_BF16 ? 2 : 4) || !aligned_to(plan, 4))
+        return RZ_ERR_ALIGN;
+    return rz_rows_embedding(make_ctx(pb, stream), ids, padding_idx, hashed, out, plan);
 }
 
-size_t rz_embedding_scratch_bytes(const rz_problem *pb) { return validate(pb) ? 0 : rz_rows_embedding_scratch(pb); }
-
-int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const void *dOut, float *dH, void *scratch,
-                          size_t scratch_bytes, void *stream)
+int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const void *dOut, float *dH, const void *plan,
+                          size_t plan_bytes, void *stream)
 {
     int st = validate(pb);
     if (st) return st;
     if (!ids || !dOut || !dH) return RZ_ERR_NULL;
-    const size_t need = rz_rows_embedding_scratch(pb);
-    if (need && !scratch) return RZ_ERR_NULL;
-    if (scratch_bytes < need) return RZ_ERR_SCRATCH;
-    if (!aligned_to(ids, 8) || !aligned_to(dOut, pb->io_dtype == RZ_BF16 ? 2 : 4) || !aligned_to(dH, 4) || !aligned_to(scratch, 4))
+    if (plan && plan_bytes < rz_rows_embedding_plan(pb)) return RZ_ERR_SCRATCH;
+    if (!aligned_to(ids, 8) || !aligned_to(dOut, pb->io_dtype == RZ_BF16 ? 2 : 4) || !aligned_to(dH, 4) || !aligned_to(plan, 4))
         return RZ_ERR_ALIGN;
     RzLaunchCtx c = make_ctx(pb, stream);
     st = zero_gradient(pb, dH, c.stream);
     if (st) return st;
-    return rz_rows_embedding_grad(c, ids, padding_idx, dOut, dH, scratch);
+    return rz_rows_embedding_grad(c, ids, padding_idx, dOut, dH, plan);
 }
 
 size_t rz_grouped_copies_bytes(const rz_problem *pb)
@@ -378,49 +379,26 @@ int rz_grouped_forward(const rz_problem *pb, int64_t groups, const int32_t *offs
     if (st) return st;
     const bool tc = use_tc_grouped(pb);
     if (!X || !Y || (tc ? !copies : !hashed)) return RZ_ERR_NULL;
-    st = check_grouped(pb, groups, offsets, X, Y, copies, copies_bytes, workspace, workspace_bytes, tc);
+    st = check_grouped(pb, groups, offsets, X, Y, copies, copies_bytes, workspace, workspace_bytes, tc, true);
     if (st) return st;
     return rz_grouped_run_forward(make_ctx(pb, stream), (int)groups, offsets, X, hashed, copies, bias, Y, workspace, tc);
 }
 
-int rz_grouped_backward_input(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *dY, const float *hashed,
-                              const void *copies, size_t copies_bytes, void *dX, void *workspace, size_t workspace_bytes, void *stream)
+int rz_grouped_backward(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const void *dY, const void *Y,
+                        const float *hashed, const void *copies, size_t copies_bytes, void *dYm, float *bias_grad, void *dX, float *dH,
+                        void *workspace, size_t workspace_bytes, void *stream)
 {
     int st = validate_groups(pb, groups);
     if (st) return st;
     const bool tc = use_tc_grouped(pb);
-    if (!dY || !dX || (tc ? !copies : !hashed)) return RZ_ERR_NULL;
-    st = check_grouped(pb, groups, offsets, dY, dX, copies, copies_bytes, workspace, workspace_bytes, tc);
+    if (!dY || (dH && !X) || (dX && (tc ? !copies : !hashed)) || (Y && !dYm) || !(bias_grad || dX || dH)) return RZ_ERR_NULL;
+    const uintptr_t element = pb->io_dtype == RZ_BF16 ? 2 : 4;
+    if (!aligned_to(dH, 4) || !aligned_to(bias_grad, 4) || !aligned_to(Y, element) || !aligned_to(dYm, tc ? 16 : element) ||
+        !aligned_to(X, dH && tc ? 16 : element))
+        return RZ_ERR_ALIGN;
+    st = check_grouped(pb, groups, offsets, dY, dX, copies, copies_bytes, workspace, workspace_bytes, tc, dX != nullptr);
     if (st) return st;
-    return rz_grouped_run_backward_input(make_ctx(pb, stream), (int)groups, offsets, dY, hashed, copies, dX, workspace, tc);
-}
-
-int rz_grouped_backward_weight(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const void *dY, float *dH,
-                               void *workspace, size_t workspace_bytes, void *stream)
-{
-    int st = validate_groups(pb, groups);
-    if (st) return st;
-    if (!X || !dY || !dH) return RZ_ERR_NULL;
-    if (!aligned_to(dH, 4)) return RZ_ERR_ALIGN;
-    const bool tc = use_tc_grouped(pb);
-    st = check_grouped(pb, groups, offsets, X, dY, nullptr, 0, workspace, workspace_bytes, tc, false);
-    if (st) return st;
-    RzLaunchCtx c = make_ctx(pb, stream);
-    st = zero_gradient(pb, dH, c.stream);
-    if (st) return st;
-    return rz_grouped_run_backward_weight(c, (int)groups, offsets, X, dY, dH, workspace, tc);
-}
-
-int rz_grouped_grad_prepare(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *dY, const void *Y, void *dYm,
-                            float *bias_grad, void *workspace, size_t workspace_bytes, void *stream)
-{
-    int st = validate_groups(pb, groups);
-    if (st) return st;
-    if (!dY || (Y && !dYm) || (!dYm && !bias_grad)) return RZ_ERR_NULL;
-    if (!aligned_to(bias_grad, 4)) return RZ_ERR_ALIGN;
-    st = check_grouped(pb, groups, offsets, dY, Y, nullptr, 0, workspace, workspace_bytes, false, false);
-    if (st) return st;
-    return rz_grouped_run_grad_prepare(make_ctx(pb, stream), (int)groups, offsets, dY, Y, dYm, bias_grad, workspace);
+    return rz_grouped_run_backward(make_ctx(pb, stream), (int)groups, offsets, X, dY, Y, hashed, copies, dYm, bias_grad, dX, dH, workspace, tc);
 }
 
 int rz_sgd_step(const rz_problem *pb, float *hashed, const float *dH, float lr, void *shadow, void *stream)

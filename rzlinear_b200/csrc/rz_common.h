@@ -85,21 +85,19 @@ int rz_tc_wait_selftest(long long limit_cycles, cudaStream_t stream);
 size_t rz_rows_sort_scratch(int64_t rows, int64_t bins);
 int rz_rows_sort_max_bins();
 int rz_rows_sort(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order, int32_t *offsets, void *scratch, cudaStream_t stream);
-int rz_rows_embedding(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const float *hashed, void *out);
-size_t rz_rows_embedding_scratch(const rz_problem *pb);
-int rz_rows_embedding_grad(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const void *dout, float *dH, void *scratch);
+int rz_rows_embedding(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const float *hashed, void *out, void *plan);
+size_t rz_rows_embedding_plan(const rz_problem *pb);
+int rz_rows_embedding_grad(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const void *dout, float *dH, const void *plan);
 
 // products grouped by row (rz_grouped.cu): pb->M rows in `groups` consecutive groups given by offsets[groups + 1] on the device
 constexpr int RZ_GROUPS_MAX = 4096;
 size_t rz_grouped_workspace(const rz_problem *pb, int groups, bool tc);
 int rz_grouped_run_forward(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *X, const float *hashed, const void *copies,
                            const float *bias, void *Y, void *ws, bool tc);
-int rz_grouped_run_backward_input(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *dY, const float *hashed,
-                                  const void *copies, void *dX, void *ws, bool tc);
-int rz_grouped_run_backward_weight(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *X, const void *dY, float *dH,
-                                   void *ws, bool tc);
-int rz_grouped_run_grad_prepare(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *dY, const void *Y, void *dYm,
-                                float *bias_grad, void *ws);
+// Y: saved output of a layer with a ReLU (dYm receives the masked gradient) or NULL; bias_grad, dX, dH: NULL where not wanted.
+// Clears bias_grad, and dH unless the call adds into it.
+int rz_grouped_run_backward(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *X, const void *dY, const void *Y,
+                            const float *hashed, const void *copies, void *dYm, float *bias_grad, void *dX, float *dH, void *ws, bool tc);
 
 int rz_simt_grouped_forward(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *X, const float *hashed, const float *bias, void *Y);
 int rz_simt_grouped_backward_input(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *dY, const float *hashed, void *dX);
@@ -115,5 +113,5 @@ int rz_tc_grouped_forward(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const
                           const float *bias, void *Y);
 int rz_tc_grouped_backward_input(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *dY,
                                  const void *copies, void *dX);
-// `maps`: {dY, X} tensor maps of each group on the device, made from rz_tc_grouped_base_maps() by the plan kernel
+// `maps`: {dY, X} tensor maps of each group, made on the device by the plan kernel
 int rz_tc_grouped_backward_weight(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *maps, float *dH);

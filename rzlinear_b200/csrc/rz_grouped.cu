@@ -13,14 +13,23 @@ namespace {
 
 constexpr int PLAN_THREADS = 1024;
 
+struct PlanList {
+    uint32_t *header;       // [0] = pieces
+    uint4 *entries;
+    uint32_t step;
+};
+
+constexpr int MAX_LISTS = 3;
+
 struct PlanArgs {
     const int32_t *offsets;
-    uint32_t groups, M, step;
-    uint32_t *header;
-    uint4 *entries;
+    uint32_t groups, M, lists;
+    PlanList list[MAX_LISTS];
     CUtensorMap *maps;      // NULL: none wanted
     uint8_t *out;           // NULL: no rows to clear
     uint64_t row_bytes;
+    float *zero[2];         // arrays to clear as a whole (NULL: none)
+    uint64_t zero_words[2];
 };
 
 // inclusive scan over the block with `op`; every thread's value and the total over the block
@@ -51,7 +60,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sums, 
     return v;
 }
 
-// Block 0 lists the pieces; the other blocks (block 0 too when it is alone) make the maps and clear rows.
+// Block b < lists writes list b; the blocks behind make the maps and clear rows (block 0 where there are none).
 __global__ void __launch_bounds__(PLAN_THREADS)
 rz_group_plan_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const PlanArgs p)
 {
@@ -75,17 +84,19 @@ rz_group_plan_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     }
     __syncthreads();
 
-    if (blockIdx.x == 0) {
+    const bool alone = gridDim.x == p.lists;
+    if (blockIdx.x < p.lists) {
+        const PlanList list = p.list[blockIdx.x];
         carry = 0;
         for (uint32_t b0 = 0; b0 < G; b0 += PLAN_THREADS) {
             const uint32_t g = b0 + tid;
             uint32_t total;
-            const uint32_t n = g < G ? (bound[g + 1] - bound[g] + p.step - 1) / p.step : 0u;
+            const uint32_t n = g < G ? (bound[g + 1] - bound[g] + list.step - 1) / list.step : 0u;
             const uint32_t before = block_scan(n, warp_sums, [](uint32_t a, uint32_t b) { return a + b; }, &total) - n;
             if (g < G) first[g] = carry + before;
             carry += total;
         }
-        if (tid == 0) p.header[0] = carry;
+        if (tid == 0) list.header[0] = carry;
         __syncthreads();
         for (uint32_t i = tid; i < carry; i += PLAN_THREADS) {
             uint32_t lo = 0, hi = G;   // the last group whose first piece is not behind i (and which has pieces)
@@ -94,12 +105,12 @@ rz_group_plan_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
                 if (first[mid] <= i) lo = mid;
                 else hi = mid;
             }
-            const uint32_t row = bound[lo] + (i - first[lo]) * p.step;
-            p.entries[i] = make_uint4(lo, row, min(row + p.step, bound[lo + 1]), 0u);
+            const uint32_t row = bound[lo] + (i - first[lo]) * list.step;
+            list.entries[i] = make_uint4(lo, row, min(row + list.step, bound[lo + 1]), 0u);
         }
-        if (gridDim.x > 1) return;
+        if (!alone || blockIdx.x) return;
     }
-    const uint32_t helper = gridDim.x > 1 ? blockIdx.x - 1 : 0, helpers = gridDim.x > 1 ? gridDim.x - 1 : 1;
+    const uint32_t helper = alone ? 0 : blockIdx.x - p.lists, helpers = alone ? 1 : gridDim.x - p.lists;
 
     if (p.maps) {
         const uint32_t dst = rzptx::smem_u32(&staged[warp]);
@@ -113,9 +124,20 @@ rz_group_plan_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
             __syncwarp();
         }
     }
+    const uint64_t step = (uint64_t)helpers * PLAN_THREADS, at = (uint64_t)helper * PLAN_THREADS + tid;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+        float *o = p.zero[z];
+        if (!o) continue;
+        const uint64_t n = p.zero_words[z];
+        const uint64_t head = min(n, (uint64_t)((16u - (uint32_t)(reinterpret_cast<uintptr_t>(o) & 15u)) & 15u) / 4), quads = (n - head) / 4;
+        if (at < head) o[at] = 0.f;
+        for (uint64_t i = at; i < quads; i += step) reinterpret_cast<float4 *>(o + head)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const uint64_t done = head + 4 * quads;
+        if (at < n - done) o[done + at] = 0.f;
+    }
     if (p.out) {
         const uint64_t head = (uint64_t)bound[0] * p.row_bytes, tail = (uint64_t)bound[G] * p.row_bytes, end = (uint64_t)p.M * p.row_bytes;
-        const uint64_t step = (uint64_t)helpers * PLAN_THREADS, at = (uint64_t)helper * PLAN_THREADS + tid;
         if (((p.row_bytes | reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0) {
             uint4 *o = reinterpret_cast<uint4 *>(p.out);
             const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -129,7 +151,7 @@ rz_group_plan_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     }
 }
 
-// ---- workspace: header, pieces, tensor maps ------------------------------------------------------------------------------
+// ---- workspace: lists (header, pieces), tensor maps -----------------------------------------------------------------------------
 constexpr uint32_t SIMT_ROWS = 64, SIMT_CHUNK = 2048;   // rows of an FMA block; rows one block of the FMA weight gradient sums
 constexpr uint32_t PREPARE_ROWS = 64;                   // rows a block of the bias pass sums
 
@@ -146,31 +168,56 @@ uint32_t step_of(const rz_problem *pb, int groups, int op, bool tc)
     return op == RZ_OP_BACKWARD_WEIGHT ? SIMT_CHUNK : SIMT_ROWS;
 }
 
-// Lists the pieces in `ws`.  `out`: rows of no group are cleared there.  `maps`: where each group's maps go, from mapA and mapB.
-int plan_pieces(const RzLaunchCtx &c, int groups, const int32_t *offsets, uint32_t step, void *ws, void *out, uint64_t row_bytes,
-                CUtensorMap *maps, const CUtensorMap *mapA, const CUtensorMap *mapB, RzGroupPieces *pieces)
-{
-    const rz_problem *pb = c.pb;
-    PlanArgs p;
-    p.offsets = offsets;
-    p.groups = (uint32_t)groups, p.M = (uint32_t)pb->M, p.step = step;
-    p.header = static_cast<uint32_t *>(ws);
-    p.entries = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(ws) + 256);
-    p.maps = maps;
-    p.out = static_cast<uint8_t *>(out), p.row_bytes = row_bytes;
-    static const CUtensorMap none = {};
-    // helper blocks: one for each 256 KB that may have to be cleared, or for each 32 maps
-    uint64_t helpers = out ? (uint64_t)pb->M * row_bytes >> 18 : 0;
-    if (maps && helpers < (uint64_t)groups / 16) helpers = (uint64_t)groups / 16;
-    if (helpers > 147) helpers = 147;
-    rz_group_plan_kernel<<<(unsigned)(1 + helpers), PLAN_THREADS, 0, c.stream>>>(mapA ? *mapA : none, mapB ? *mapB : none, p);
-    rz_count_launch(1);
-    pieces->header = p.header;
-    pieces->entries = p.entries;
-    pieces->most = most_pieces(pb, groups, step);
-    pieces->group_tiles = (uint32_t)((pb->K + pb->BK - 1) / pb->BK);
-    return rz_record_cuda(cudaGetLastError(), "group plan launch");
-}
+// A plan under construction: lists are added one behind the other in the workspace, then one launch writes them all.
+struct Plan {
+    const RzLaunchCtx &c;
+    int groups;
+    uint8_t *ws;
+    size_t used = 0;
+    PlanArgs args = {};
+    CUtensorMap mapA = {}, mapB = {};
+
+    Plan(const RzLaunchCtx &c_, int groups_, const int32_t *offsets, void *ws_) : c(c_), groups(groups_), ws(static_cast<uint8_t *>(ws_))
+    {
+        args.offsets = offsets;
+        args.groups = (uint32_t)groups_, args.M = (uint32_t)c_.pb->M;
+    }
+    RzGroupPieces add(uint32_t step)
+    {
+        RzGroupPieces pieces;
+        PlanList &l = args.list[args.lists++];
+        l.step = step;
+        l.header = reinterpret_cast<uint32_t *>(ws + used);
+        l.entries = reinterpret_cast<uint4 *>(ws + used + 256);
+        used += pieces_bytes(c.pb, groups, step);
+        pieces.header = l.header, pieces.entries = l.entries;
+        pieces.most = most_pieces(c.pb, groups, step);
+        pieces.group_tiles = (uint32_t)((c.pb->K + c.pb->BK - 1) / c.pb->BK);
+        return pieces;
+    }
+    // each group's maps of dY (mapA) and X (mapB)
+    CUtensorMap *add_maps()
+    {
+        args.maps = reinterpret_cast<CUtensorMap *>(ws + used);
+        used += 2 * sizeof(CUtensorMap) * (size_t)groups;
+        return args.maps;
+    }
+    void zero(int z, float *words, uint64_t n) { args.zero[z] = words, args.zero_words[z] = n; }
+    // rows of `out` that belong to no group are cleared
+    void clear(void *out, uint64_t row_bytes) { args.out = static_cast<uint8_t *>(out), args.row_bytes = row_bytes; }
+    int launch()
+    {
+        // helper blocks: one for each 256 KB of rows that may have to be cleared, each 64 KB of an array, each 32 maps
+        uint64_t helpers = args.out ? (uint64_t)args.M * args.row_bytes >> 18 : 0;
+        const uint64_t arrays = (args.zero_words[0] + args.zero_words[1]) >> 14;
+        if (helpers < arrays) helpers = arrays;
+        if (args.maps && helpers < (uint64_t)groups / 16) helpers = (uint64_t)groups / 16;
+        if (helpers > 147) helpers = 147;
+        rz_group_plan_kernel<<<(unsigned)(args.lists + helpers), PLAN_THREADS, 0, c.stream>>>(mapA, mapB, args);
+        rz_count_launch(1);
+        return rz_record_cuda(cudaGetLastError(), "group plan launch");
+    }
+};
 
 // ---- bias gradient and ReLU mask -----------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f32(T v);
@@ -237,73 +284,69 @@ uint64_t element_bytes(const rz_problem *pb) { return pb->io_dtype == RZ_BF16 ? 
 
 size_t rz_grouped_workspace(const rz_problem *pb, int groups, bool tc)
 {
-    // one size for all operations of a layer: the longest list (the bias pass has one too), then the weight gradient's maps
-    size_t most = pieces_bytes(pb, groups, PREPARE_ROWS);
-    for (int op = RZ_OP_FORWARD; op <= RZ_OP_BACKWARD_WEIGHT; ++op) {
-        const size_t b = pieces_bytes(pb, groups, step_of(pb, groups, op, tc));
-        if (b > most) most = b;
-    }
-    return most + (tc ? 2 * sizeof(CUtensorMap) * (size_t)groups : 0);
+    // the backward's three lists and the weight gradient's maps, or the forward's list
+    const size_t forward = pieces_bytes(pb, groups, step_of(pb, groups, RZ_OP_FORWARD, tc));
+    const size_t backward = pieces_bytes(pb, groups, PREPARE_ROWS) + pieces_bytes(pb, groups, step_of(pb, groups, RZ_OP_BACKWARD_INPUT, tc)) +
+                            pieces_bytes(pb, groups, step_of(pb, groups, RZ_OP_BACKWARD_WEIGHT, tc)) +
+                            (tc ? 2 * sizeof(CUtensorMap) * (size_t)groups : 0);
+    return forward > backward ? forward : backward;
 }
 
 int rz_grouped_run_forward(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *X, const float *hashed, const void *copies,
                            const float *bias, void *Y, void *ws, bool tc)
 {
-    RzGroupPieces pieces;
-    int st = plan_pieces(c, groups, offsets, step_of(c.pb, groups, RZ_OP_FORWARD, tc), ws, Y, element_bytes(c.pb) * (uint64_t)c.pb->N, nullptr,
-                         nullptr, nullptr, &pieces);
+    Plan plan(c, groups, offsets, ws);
+    const RzGroupPieces pieces = plan.add(step_of(c.pb, groups, RZ_OP_FORWARD, tc));
+    plan.clear(Y, element_bytes(c.pb) * (uint64_t)c.pb->N);
+    const int st = plan.launch();
     if (st) return st;
     if (tc) return rz_tc_grouped_forward(c, rz_tc_grouped_plan(c.pb, groups, RZ_OP_FORWARD), pieces, X, copies, bias, Y);
     return rz_simt_grouped_forward(c, pieces, X, hashed, bias, Y);
 }
 
-int rz_grouped_run_backward_input(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *dY, const float *hashed,
-                                  const void *copies, void *dX, void *ws, bool tc)
-{
-    RzGroupPieces pieces;
-    int st = plan_pieces(c, groups, offsets, step_of(c.pb, groups, RZ_OP_BACKWARD_INPUT, tc), ws, dX, element_bytes(c.pb) * (uint64_t)c.pb->K,
-                         nullptr, nullptr, nullptr, &pieces);
-    if (st) return st;
-    if (tc) return rz_tc_grouped_backward_input(c, rz_tc_grouped_plan(c.pb, groups, RZ_OP_BACKWARD_INPUT), pieces, dY, copies, dX);
-    return rz_simt_grouped_backward_input(c, pieces, dY, hashed, dX);
-}
-
-int rz_grouped_run_backward_weight(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *X, const void *dY, float *dH,
-                                   void *ws, bool tc)
+int rz_grouped_run_backward(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *X, const void *dY, const void *Y,
+                            const float *hashed, const void *copies, void *dYm, float *bias_grad, void *dX, float *dH, void *ws, bool tc)
 {
     const rz_problem *pb = c.pb;
-    RzGroupPieces pieces;
-    if (!tc) {
-        int st = plan_pieces(c, groups, offsets, SIMT_CHUNK, ws, nullptr, 0, nullptr, nullptr, nullptr, &pieces);
-        if (st) return st;
-        return rz_simt_grouped_backward_weight(c, pieces, X, dY, dH);
-    }
-    const rztc::Geometry g = rztc::geometry(pb);
-    const bool tf32 = pb->precision != RZ_PREC_BF16;
-    CUtensorMap mapA, mapB;   // A = dY, B = X, boxes of one 128-byte row by a stage's contraction rows
-    int st = rztc::map_matrix(&mapA, tf32, true, dY, pb->M, pb->N, g.epr, g.epr);
-    if (st) return st;
-    st = rztc::map_matrix(&mapB, tf32, true, X, pb->M, pb->K, g.epr, g.epr);
-    if (st) return st;
-    const RzTcGroupPlan plan = rz_tc_grouped_plan(pb, groups, RZ_OP_BACKWARD_WEIGHT);
-    static_assert(sizeof(CUtensorMap) == 128, "tensor maps are 128 bytes");   // (they stand behind the list)
-    CUtensorMap *maps = reinterpret_cast<CUtensorMap *>(static_cast<uint8_t *>(ws) + (rz_grouped_workspace(pb, groups, true) - 2 * sizeof(CUtensorMap) * (size_t)groups));
-    st = plan_pieces(c, groups, offsets, plan.step, ws, nullptr, 0, maps, &mapA, &mapB, &pieces);
-    if (st) return st;
-    return rz_tc_grouped_backward_weight(c, plan, pieces, maps, dH);
-}
-
-int rz_grouped_run_grad_prepare(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *dY, const void *Y, void *dYm,
-                                float *bias_grad, void *ws)
-{
-    RzGroupPieces pieces;
+    static_assert(sizeof(CUtensorMap) == 128, "tensor maps are 128 bytes");
+    const bool prepare = Y || bias_grad;
+    const void *grad = Y ? dYm : dY;   // what the products see
+    Plan plan(c, groups, offsets, ws);
+    RzGroupPieces rows, blocks, chunks;
     int st;
-    if (bias_grad) {
-        st = rz_record_cuda(cudaMemsetAsync(bias_grad, 0, sizeof(float) * (size_t)groups * (size_t)c.pb->N, c.stream), "zero bias gradient");
+    if (prepare) rows = plan.add(PREPARE_ROWS);
+    if (dX) {
+        blocks = plan.add(step_of(pb, groups, RZ_OP_BACKWARD_INPUT, tc));
+        plan.clear(dX, element_bytes(pb) * (uint64_t)pb->K);
+    }
+    const CUtensorMap *maps = nullptr;
+    if (dH) {
+        chunks = plan.add(step_of(pb, groups, RZ_OP_BACKWARD_WEIGHT, tc));
+        if (tc) {   // A = dY, B = X, boxes of one 128-byte row by a stage's contraction rows
+            const rztc::Geometry g = rztc::geometry(pb);
+            const bool tf32 = pb->precision != RZ_PREC_BF16;
+            st = rztc::map_matrix(&plan.mapA, tf32, true, grad, pb->M, pb->N, g.epr, g.epr);
+            if (st) return st;
+            st = rztc::map_matrix(&plan.mapB, tf32, true, X, pb->M, pb->K, g.epr, g.epr);
+            if (st) return st;
+            maps = plan.add_maps();
+        }
+    }
+    if (bias_grad) plan.zero(0, bias_grad, (uint64_t)groups * (uint64_t)pb->N);
+    if (dH && !(pb->flags & RZ_FLAG_ACCUMULATE_DH)) plan.zero(1, dH, (uint64_t)pb->H);
+    st = plan.launch();
+    if (st) return st;
+    if (prepare) {
+        st = pb->io_dtype == RZ_BF16 ? launch_prepare<__nv_bfloat16>(c, rows, dY, Y, dYm, bias_grad)
+                                     : launch_prepare<float>(c, rows, dY, Y, dYm, bias_grad);
         if (st) return st;
     }
-    st = plan_pieces(c, groups, offsets, PREPARE_ROWS, ws, nullptr, 0, nullptr, nullptr, nullptr, &pieces);
-    if (st) return st;
-    if (c.pb->io_dtype == RZ_BF16) return launch_prepare<__nv_bfloat16>(c, pieces, dY, Y, dYm, bias_grad);
-    return launch_prepare<float>(c, pieces, dY, Y, dYm, bias_grad);
+    if (dX) {
+        st = tc ? rz_tc_grouped_backward_input(c, rz_tc_grouped_plan(pb, groups, RZ_OP_BACKWARD_INPUT), blocks, grad, copies, dX)
+                : rz_simt_grouped_backward_input(c, blocks, grad, hashed, dX);
+        if (st) return st;
+    }
+    if (!dH) return RZ_OK;
+    if (tc) return rz_tc_grouped_backward_weight(c, rz_tc_grouped_plan(pb, groups, RZ_OP_BACKWARD_WEIGHT), chunks, maps, dH);
+    return rz_simt_grouped_backward_weight(c, chunks, X, grad, dH);
 }

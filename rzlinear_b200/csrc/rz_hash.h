@@ -60,3 +60,58 @@ RZ_HD uint64_t rz_tile_offset(const RzHash &h, uint32_t pk, uint32_t pn)
     }
     return rz_fastmod(a, h.range, h.m_range);
 }
+
+// The same offsets in 32-bit arithmetic where the sizes allow it, for kernels that hash about as often as they load: a 64-bit
+// modulus costs some 40 instructions, a 32-bit one 4.  `linear32`: the residues of R make both linear forms fit 32 bits for every tile
+// of the matrix (the default prime 45007, up to about 95000 tile rows).  `square32`: R0^2 <= 2^32, so the combined two-level value
+// fits; a single-level value always does.  v mod d as in rz_fastmod, with m = floor((2^32 - 1) / d).
+struct RzHash32 {
+    uint32_t R0, R1, R2, R3, R4, R5, R7;   // residues mod R0
+    uint32_t m_R0, range, m_range;
+    uint32_t linear32, square32;
+};
+
+RZ_HD uint32_t rz_mulhi32(uint32_t a, uint32_t b)
+{
+#if defined(__CUDA_ARCH__)
+    return __umulhi(a, b);
+#else
+    return (uint32_t)(((uint64_t)a * b) >> 32);
+#endif
+}
+
+RZ_HD uint32_t rz_fastmod32(uint32_t v, uint32_t d, uint32_t m)
+{
+    const uint32_t r = v - rz_mulhi32(v, m) * d;
+    return r >= d ? r - d : r;
+}
+
+// tiles (pk, pn) with pk < tile_rows and pn < tile_cols
+inline RzHash32 rz_hash32(const RzHash &h, uint64_t tile_rows, uint64_t tile_cols)
+{
+    RzHash32 s;
+    s.R0 = (uint32_t)h.R0;
+    s.R1 = (uint32_t)(h.R1 % h.R0), s.R2 = (uint32_t)(h.R2 % h.R0), s.R3 = (uint32_t)(h.R3 % h.R0);
+    s.R4 = (uint32_t)(h.R4 % h.R0), s.R5 = (uint32_t)(h.R5 % h.R0), s.R7 = (uint32_t)(h.R7 % h.R0);
+    s.m_R0 = 0xffffffffu / s.R0;
+    s.range = (uint32_t)h.range;
+    s.m_range = 0xffffffffu / s.range;
+    const uint64_t lim = (uint64_t)1 << 32, pk = tile_rows - 1, pn = tile_cols - 1;   // (all factors are below 2^31)
+    s.linear32 = pk * s.R3 + pn * s.R2 + s.R1 < lim && (!h.two_level || pk * s.R7 + pn * s.R5 + s.R4 < lim);
+    s.square32 = !h.two_level || h.R0 * h.R0 <= lim;
+    return s;
+}
+
+RZ_HD uint32_t rz_tile_offset32(const RzHash &h, const RzHash32 &s, uint32_t pk, uint32_t pn)
+{
+    uint32_t a, b = 0;
+    if (s.linear32) {
+        a = rz_fastmod32(pk * s.R3 + pn * s.R2 + s.R1, s.R0, s.m_R0);
+        if (h.two_level) b = rz_fastmod32(pk * s.R7 + pn * s.R5 + s.R4, s.R0, s.m_R0);
+    } else {
+        a = (uint32_t)rz_fastmod((uint64_t)pk * s.R3 + (uint64_t)pn * s.R2 + s.R1, h.R0, h.m_R0);
+        if (h.two_level) b = (uint32_t)rz_fastmod((uint64_t)pk * s.R7 + (uint64_t)pn * s.R5 + s.R4, h.R0, h.m_R0);
+    }
+    if (s.square32) return rz_fastmod32(h.two_level ? a * s.R0 + b : a, s.range, s.m_range);
+    return (uint32_t)rz_fastmod((uint64_t)a * s.R0 + b, h.range, h.m_range);
+}

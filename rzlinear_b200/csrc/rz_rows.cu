@@ -1,5 +1,5 @@
-// Rows picked by an index: stable counting sort of row keys, embedding lookup in a virtual table, and the lookup's
-// gradient by sorted tokens.
+// Rows picked by an index: stable counting sort of row keys, embedding lookup in a virtual table, and the lookup's gradient,
+// token by token.
 //
 // The table is a virtual weight W[V, D] like any other of this library: row k is cut into segments of BN columns, and
 // segment pn of row k is the contiguous run of words  hashed[ off(k / BK, pn) + (k % BK) * BN ... + BN ).
@@ -7,6 +7,10 @@
 // Every kernel here is bound by memory or by the reductions into the hashed gradient, so they are plain SIMT kernels: what
 // matters is that every request is a full 128-byte line of consecutive words, that a hash (about 60 integer instructions) is
 // computed by 32 lanes for 32 segments at once, and that few launches are made.
+#include <atomic>
+#include <cstring>
+#include <type_traits>
+
 #include "rz_common.h"
 
 namespace {
@@ -23,6 +27,11 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 __device__ __forceinline__ void store_pair(float *p, float a, float b) { *reinterpret_cast<float2 *>(p) = make_float2(a, b); }
 __device__ __forceinline__ void store_pair(__nv_bfloat16 *p, float a, float b) { *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(a, b); }
 
+__device__ __forceinline__ void red_pair(float *p, float a, float b)
+{
+    asm volatile("red.global.add.v2.f32 [%0], {%1, %2};" ::"l"(p), "f"(a), "f"(b) : "memory");
+}
+
 // A token that selects a row of the table: inside [0, V) and not the padding row.
 __device__ __forceinline__ bool live_id(int64_t id, uint32_t V, int64_t padding) { return id >= 0 && id < (int64_t)V && id != padding; }
 
@@ -37,6 +46,17 @@ __device__ __forceinline__ bool live_id(int64_t id, uint32_t V, int64_t padding)
 constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32, SORT_ITEMS = 4;
 constexpr int SORT_TILE = SORT_THREADS * SORT_ITEMS;
 constexpr int SORT_MAX_BINS = 1024, SORT_MAX_BLOCKS = 148;
+
+// Lanes whose `bits` low key bits equal this lane's, one vote per bit.
+__device__ __forceinline__ uint32_t same_key(uint32_t key, int bits)
+{
+    uint32_t same = FULL;
+    for (int b = 0; b < bits; ++b) {
+        const uint32_t set = __ballot_sync(FULL, (key >> b) & 1u);
+        same &= (key >> b) & 1u ? set : ~set;
+    }
+    return same;
+}
 
 __device__ __forceinline__ uint32_t sort_bin(const int64_t *__restrict__ keys, uint32_t row, uint32_t bins)
 {
@@ -88,7 +108,7 @@ __device__ __forceinline__ uint32_t block_exclusive_scan(uint32_t v, uint32_t *w
 // `hist` NULL: one block, one tile.
 __global__ void __launch_bounds__(SORT_THREADS)
 rz_sort_place_kernel(const int64_t *__restrict__ keys, uint32_t rows, uint32_t bins, uint32_t rows_per_block,
-                     const uint32_t *__restrict__ hist, int32_t *__restrict__ order, int32_t *__restrict__ offsets)
+                     int bits, const uint32_t *__restrict__ hist, int32_t *__restrict__ order, int32_t *__restrict__ offsets)
 {
     extern __shared__ uint32_t sort_smem[];
     __shared__ uint32_t warp_sums[SORT_WARPS];
@@ -131,7 +151,7 @@ rz_sort_place_kernel(const int64_t *__restrict__ keys, uint32_t rows, uint32_t b
         uint32_t *mine = count + warp * nb;
 #pragma unroll
         for (int j = 0; j < SORT_ITEMS; ++j) {
-            const uint32_t same = __match_any_sync(FULL, bin[j]);
+            const uint32_t same = same_key(bin[j], bits);   // (`bits` hold every bin, and a value for the slots behind the rows)
             const uint32_t leader = __ffs(same) - 1;
             uint32_t old = 0;
             if (lane == leader && bin[j] != FULL) {
@@ -191,7 +211,7 @@ rz_sort_place_kernel(const int64_t *__restrict__ keys, uint32_t rows, uint32_t b
 template <typename T, bool PAIRS>
 __global__ void __launch_bounds__(256)
 rz_embedding_kernel(const int64_t *__restrict__ ids, int64_t padding, const float *__restrict__ hashed, T *__restrict__ out,
-                    RzHash hash, uint64_t total, uint32_t V, uint32_t D, uint32_t nn, uint32_t per_warp, float alpha)
+                    RzHash hash, RzHash32 hash32, uint64_t total, uint32_t V, uint32_t D, uint32_t nn, uint32_t per_warp, float alpha)
 {
     const uint32_t lane = threadIdx.x & 31;
     const uint64_t stride = (uint64_t)gridDim.x * (blockDim.x / 32) * per_warp;
@@ -210,7 +230,7 @@ rz_embedding_kernel(const int64_t *__restrict__ ids, int64_t padding, const floa
             len = min(BN, D - pn * BN);
             if (live) {
                 const uint32_t k = (uint32_t)id, pk = k / BK;
-                src = rz_tile_offset(hash, pk, pn) + (uint64_t)(k - pk * BK) * BN;
+                src = rz_tile_offset32(hash, hash32, pk, pn) + (uint64_t)(k - pk * BK) * BN;
             }
         }
 #pragma unroll 4
@@ -228,21 +248,74 @@ rz_embedding_kernel(const int64_t *__restrict__ ids, int64_t padding, const floa
             }
         }
     }
+    // a token sort may run beside this kernel: the grid ends after it does.  (One block waits; if all did, the ones not yet
+    // started would wait for those that had finished.)
+    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// The same for hash tiles and rows of whole 64-word pieces: a unit is 64 words, so every unit is full, its place in the output
+// is its number, and what the copy loop fetches from the hashing lane is one 32-bit word.
+template <typename T>
+__global__ void __launch_bounds__(256)
+rz_embedding_pieces_kernel(const int64_t *__restrict__ ids, int64_t padding, const float *__restrict__ hashed, T *__restrict__ out,
+                           RzHash hash, RzHash32 hash32, uint64_t total, uint32_t V, uint32_t per_row, uint32_t per_warp, float alpha)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t stride = (uint64_t)gridDim.x * (blockDim.x / 32) * per_warp;
+    const uint32_t BN = (uint32_t)hash.BN, BK = (uint32_t)hash.BK;
+    for (uint64_t u0 = ((uint64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5)) * per_warp; u0 < total; u0 += stride) {
+        const uint32_t n = (uint32_t)min((uint64_t)per_warp, total - u0);
+        uint32_t src = FULL;   // (no word has this number)
+        if (lane < n) {
+            const uint64_t u = u0 + lane, t = u / per_row;
+            const uint32_t col = (uint32_t)(u - t * per_row) * 64, pn = col / BN;
+            const int64_t id = ids[t];
+            if (live_id(id, V, padding)) {
+                const uint32_t k = (uint32_t)id, pk = k / BK;
+                src = rz_tile_offset32(hash, hash32, pk, pn) + (k - pk * BK) * BN + (col - pn * BN);
+            }
+        }
+        T *dst = out + u0 * 64 + 2 * lane;
+        constexpr int U = 8;
+        for (uint32_t j0 = 0; j0 < n; j0 += U) {
+            float a[U], b[U];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const uint32_t s = __shfl_sync(FULL, src, j0 + j);   // (lanes from n on hold FULL)
+                a[j] = b[j] = 0.f;
+                if (s != FULL) {
+                    const float *w = hashed + s + 2 * lane;
+                    a[j] = __ldg(w), b[j] = __ldg(w + 1);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+                if (j0 + j < n) store_pair(dst + (size_t)(j0 + j) * 64, a[j] * alpha, b[j] * alpha);
+        }
+    }
+    // a token sort may run beside this kernel: the grid ends after it does.  (One block waits; if all did, the ones not yet
+    // started would wait for those that had finished.)
+    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---- embedding gradient -----------------------------------------------------------------------------------------------
 // dH[word of (k, n)] += alpha * sum over the tokens t with ids[t] = k of dOut[t, n].
 //
 // A token that occurs often would add the same words over and over, and reductions (1.3e12 a second at best, whatever their
-// width) cost more than reading: 2 bytes at 6.5 TB/s are 3.3e12 elements a second.  So chunks of the batch are sorted by
-// token first, runs of one token are summed in registers in 32 bits, and one reduction per word and run is made.  Sorting
-// within chunks is one launch, needs no exchange between blocks and finds nearly all repetitions (a token that returns in
-// another chunk costs one more reduction per word).
+// width) cost more than reading: 2 bytes at 6.5 TB/s are 3.3e12 elements a second.  So the tokens are brought together first: runs
+// of one token are then summed in registers in 32 bits, and one reduction per word and run is made.
+//
+// One CTA sorts a chunk of up to 16384 tokens (least significant digits first, digits of up to 8 bits, ranks from votes; a warp-wide
+// match instruction takes some 180 cycles of the SM), which finds nearly all repetitions: a token that returns in another chunk
+// costs one more reduction per word.  The sort is slow - 17 us for 8192 tokens, all latency - but needs nothing of the gradient, so the
+// forward call makes it, on a few SMs beside the lookup, which takes the others.
+// (Instead, one launch in the backward: a cluster of eight CTAs counting chunks of 32768 tokens in a hash table in its shared memory
+// took 31 us for 16384 tokens, a table in L2 19 us and, for 131072 tokens, 112 us.)
 constexpr int CHUNK_THREADS = 1024, CHUNK_WARPS = 32;
 
 template <int ITEMS>
 __global__ void __launch_bounds__(CHUNK_THREADS)
-rz_token_sort_kernel(const int64_t *__restrict__ ids, int64_t padding, uint32_t T, uint32_t V, int passes,
+rz_token_sort_kernel(const int64_t *__restrict__ ids, int64_t padding, uint32_t T, uint32_t V, int passes, int width,
                      uint32_t *__restrict__ sorted_id, uint32_t *__restrict__ sorted_row)
 {
     constexpr uint32_t CHUNK = CHUNK_THREADS * ITEMS;
@@ -251,7 +324,8 @@ rz_token_sort_kernel(const int64_t *__restrict__ ids, int64_t padding, uint32_t 
     uint32_t *count = skey + CHUNK;                                               // [CHUNK_WARPS][256]
     uint16_t *spos = reinterpret_cast<uint16_t *>(count + CHUNK_WARPS * 256);     // [CHUNK]
     __shared__ uint32_t warp_sums[32];
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.launch_dependents;");   // the lookup runs beside this kernel, and waits for it at its end
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1u << width;
     const uint32_t begin = blockIdx.x * CHUNK, valid = min(CHUNK, T - begin);
     const uint32_t first = warp * (32 * ITEMS) + lane;
     uint32_t key[ITEMS], pos[ITEMS], rank[ITEMS];
@@ -272,8 +346,8 @@ rz_token_sort_kernel(const int64_t *__restrict__ ids, int64_t padding, uint32_t 
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) {
-            const uint32_t d = (key[j] >> (8 * p)) & 255u;
-            const uint32_t same = __match_any_sync(FULL, d);
+            const uint32_t d = (key[j] >> (width * p)) & (digits - 1u);
+            const uint32_t same = same_key(d, width);
             const uint32_t leader = __ffs(same) - 1;
             uint32_t old = 0;
             if (lane == leader) {
@@ -285,7 +359,7 @@ rz_token_sort_kernel(const int64_t *__restrict__ ids, int64_t padding, uint32_t 
         }
         __syncthreads();
         uint32_t sum = 0;
-        if (threadIdx.x < 256) {
+        if (threadIdx.x < digits) {
 #pragma unroll 8
             for (int w = 0; w < CHUNK_WARPS; ++w) {
                 const uint32_t v = count[w * 256 + threadIdx.x];
@@ -295,14 +369,14 @@ rz_token_sort_kernel(const int64_t *__restrict__ ids, int64_t padding, uint32_t 
         }
         uint32_t total;
         const uint32_t at = block_exclusive_scan(sum, warp_sums, CHUNK_WARPS, &total);
-        if (threadIdx.x < 256) {
+        if (threadIdx.x < digits) {
 #pragma unroll 8
             for (int w = 0; w < CHUNK_WARPS; ++w) count[w * 256 + threadIdx.x] += at;
         }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) {
-            const uint32_t dst = mine[(key[j] >> (8 * p)) & 255u] + rank[j];
+            const uint32_t dst = mine[(key[j] >> (width * p)) & (digits - 1u)] + rank[j];
             skey[dst] = key[j];
             spos[dst] = (uint16_t)pos[j];
         }
@@ -324,169 +398,327 @@ rz_token_sort_kernel(const int64_t *__restrict__ ids, int64_t padding, uint32_t 
     }
 }
 
-// A warp takes 32 consecutive places of the sorted batch and 64 columns: lane l sums columns c0 + l and c0 + 32 + l, so that a
-// reduction instruction covers 32 consecutive words.  ALIGNED (BN a multiple of 32): each half lies in one segment, and
-// lane i hashes place i's segments for the whole warp; otherwise every lane hashes its own columns at the end of a run.
-// PACKED (bf16, even rows): one 4-byte load brings columns c0 + 2l and c0 + 2l + 1, exchanged between the lanes at the end of a
-// run.  `sorted_id` NULL: places are the tokens themselves (batches too short to be worth sorting).
-template <typename T, bool ALIGNED, bool PACKED>
-__global__ void __launch_bounds__(256)
+// The 32 places of the sorted batch that a warp works on: lane i holds place i's table row and row of dOut.
+struct Places {
+    uint32_t id, row, live, ends;   // (live, ends: masks over the places; ends = last place of a run of one token)
+};
+
+// `sorted_id` NULL: places are the tokens themselves (batches too short to be worth sorting).
+__device__ __forceinline__ Places load_places(const int64_t *__restrict__ ids, int64_t padding, const uint32_t *__restrict__ sorted_id,
+                                              const uint32_t *__restrict__ sorted_row, uint32_t block, uint32_t T, uint32_t V)
+{
+    const uint32_t lane = threadIdx.x & 31, place = block * 32 + lane;
+    Places p;
+    p.id = V, p.row = 0;
+    if (place < T) {
+        if (sorted_id) {
+            p.id = sorted_id[place];
+            p.row = sorted_row[place];
+        } else {
+            const int64_t v = ids[place];
+            p.id = live_id(v, V, padding) ? (uint32_t)v : V;
+            p.row = place;
+        }
+    }
+    p.live = __ballot_sync(FULL, p.id < V);
+    const uint32_t next = __shfl_down_sync(FULL, p.id, 1);
+    p.ends = __ballot_sync(FULL, lane == 31 || next != p.id);
+    return p;
+}
+
+// Two neighbouring elements as they are loaded, and their values.
+template <typename T> struct Pair;
+template <> struct Pair<float> {
+    float2 v = make_float2(0.f, 0.f);
+    __device__ __forceinline__ void load(const float *p) { v = __ldg(reinterpret_cast<const float2 *>(p)); }
+    __device__ __forceinline__ float first() const { return v.x; }
+    __device__ __forceinline__ float second() const { return v.y; }
+};
+template <> struct Pair<__nv_bfloat16> {
+    uint32_t v = 0;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { v = __ldg(reinterpret_cast<const uint32_t *>(p)); }
+    __device__ __forceinline__ float first() const { return __uint_as_float(v << 16); }
+    __device__ __forceinline__ float second() const { return __uint_as_float(v & 0xffff0000u); }
+};
+
+// Whole hash-tile columns of 32 and rows of pairs: a warp takes 32 places and S pieces of 64 columns, lane l columns 2l and 2l + 1 of
+// each piece (one load).  The words of a piece are consecutive (WHOLE: hash tiles of 64 columns and their multiples), or those of
+// either half of it are, and begin anywhere: where they begin at an even word the pairs are reduced as they are, elsewhere each
+// lane takes its left neighbour's second value and the first and the last word go alone.  Lane i hashes place i's tiles for the
+// whole warp.  What a place costs by itself - its row, its tests - is shared by S pieces.
+// 16384 x 4096 bf16, 9 in 10 tokens live, text: 43 us with S = 2 in blocks of 128 threads; 50 with S = 1 and 53 with S = 4 (blocks
+// of 256: 54).  With neither reductions nor reads from DRAM it takes 40 with S = 4: latency and issue slots bound it as much as
+// the 36 M words it adds (34 us at the 1.06e12 a second that rows of 64 words at random places reach) and the 130 MB it reads (20 us).
+constexpr int GRAD_THREADS = 128;
+
+template <typename T, int S, bool WHOLE>
+__global__ void __launch_bounds__(GRAD_THREADS)
+rz_embedding_grad_pairs_kernel(const int64_t *__restrict__ ids, int64_t padding, const uint32_t *__restrict__ sorted_id,
+                               const uint32_t *__restrict__ sorted_row, const T *__restrict__ dout, float *__restrict__ dH, RzHash hash, RzHash32 hash32,
+                               uint32_t T_, uint32_t V, uint32_t D, uint32_t colblocks, uint64_t units, float alpha)
+{
+    constexpr int RUNS = WHOLE ? 1 : 2, LANES = 32 / RUNS;   // runs of consecutive words in a piece, lanes of one
+    const uint32_t lane = threadIdx.x & 31, run = lane / LANES, in_run = lane % LANES;
+    const uint64_t unit = (uint64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
+    if (unit >= units) return;
+    const uint32_t block = (uint32_t)(unit / colblocks), c0 = (uint32_t)(unit - (uint64_t)block * colblocks) * (64 * S);
+    const uint32_t BN = (uint32_t)hash.BN, BK = (uint32_t)hash.BK;
+    const Places p = load_places(ids, padding, sorted_id, sorted_row, block, T_, V);
+    if (!p.live) return;
+    uint32_t dst[S][RUNS];   // first word of this lane's place in each run
+    {
+        const uint32_t pk = p.id / BK, k_in = p.id - pk * BK;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int r = 0; r < RUNS; ++r) {
+                const uint32_t col = c0 + s * 64 + r * 32, pn = col / BN;
+                dst[s][r] = p.id < V && col < D ? rz_tile_offset32(hash, hash32, pk, pn) + k_in * BN + (col - pn * BN) : 0u;
+            }
+    }
+    const T *src = dout + c0 + 2 * lane;
+    float *const base = dH + 2 * in_run;
+    float a[S], b[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) a[s] = b[s] = 0.f;
+    constexpr int U = S * sizeof(T) >= 16 ? 4 : 8;   // places whose loads are in flight together
+
+    // ALL: all 64 S columns exist, and all 32 places have a token
+    auto add_places = [&](auto all) {
+        constexpr bool ALL = decltype(all)::value;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32; i0 += U) {
+            const uint32_t live = p.live >> i0, ends = p.ends >> i0;
+            if (!ALL && (live & ((1u << U) - 1u)) == 0) continue;
+            Pair<T> v[U][S];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const T *at = src + (size_t)__shfl_sync(FULL, p.row, i0 + i) * D;
+                if (ALL || ((live >> i) & 1u)) {
+#pragma unroll
+                    for (int s = 0; s < S; ++s)
+                        if (ALL || c0 + s * 64 + 2 * lane < D) v[i][s].load(at + s * 64);   // (rows are pairs)
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+#pragma unroll
+                for (int s = 0; s < S; ++s) a[s] += v[i][s].first(), b[s] += v[i][s].second();
+                if (!((ends >> i) & 1u)) continue;
+                if (ALL || ((live >> i) & 1u)) {
+#pragma unroll
+                    for (int s = 0; s < S; ++s) {
+                        if (!ALL && c0 + s * 64 >= D) break;
+                        uint32_t d = __shfl_sync(FULL, dst[s][0], i0 + i);
+                        if (!WHOLE) {
+                            const uint32_t d1 = __shfl_sync(FULL, dst[s][RUNS - 1], i0 + i);
+                            if (run) d = d1;
+                        }
+                        // columns of this run that exist
+                        const uint32_t col = c0 + s * 64 + run * 32;
+                        const uint32_t width = ALL ? 2 * LANES : min(D - min(col, D), 2u * LANES);
+                        float *word = base + d;
+                        const float x = a[s] * alpha, y = b[s] * alpha;
+                        if (WHOLE ? (d & 1u) : __any_sync(0xffffffffu, d & 1u)) {
+                            const float left = __shfl_up_sync(FULL, y, 1);
+                            const bool odd = d & 1u, first = in_run == 0, last = 2 * in_run + 2 == width;
+                            if (2 * in_run < width && !(odd && first)) red_pair(word - odd, odd ? left : x, odd ? x : y);
+                            if (odd && width && (first || last)) atomicAdd(word + !first, first ? x : y);
+                            if (odd && first && last) atomicAdd(word + 1, y);   // (a run of two columns)
+                        } else if (ALL || 2 * in_run < width) {
+                            red_pair(word, x, y);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < S; ++s) a[s] = b[s] = 0.f;
+            }
+        }
+    };
+    if (c0 + 64 * S <= D && p.live == FULL) add_places(std::true_type());
+    else add_places(std::false_type());
+}
+
+// Any hash tile, row length and alignment: a warp takes 32 places and up to 64 columns of one segment, lane l columns l and 32 + l of
+// them, so that a reduction instruction covers 32 consecutive words.
+template <typename T>
+__global__ void __launch_bounds__(GRAD_THREADS)
 rz_embedding_grad_kernel(const int64_t *__restrict__ ids, int64_t padding, const uint32_t *__restrict__ sorted_id,
-                         const uint32_t *__restrict__ sorted_row, const T *__restrict__ dout, float *__restrict__ dH, RzHash hash,
+                         const uint32_t *__restrict__ sorted_row, const T *__restrict__ dout, float *__restrict__ dH, RzHash hash, RzHash32 hash32,
                          uint32_t T_, uint32_t V, uint32_t D, uint32_t colblocks, uint64_t units, float alpha)
 {
     const uint32_t lane = threadIdx.x & 31;
     const uint64_t unit = (uint64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
     if (unit >= units) return;
-    const uint32_t pb = (uint32_t)(unit / colblocks), cb = (uint32_t)(unit - (uint64_t)pb * colblocks);
+    const uint32_t block = (uint32_t)(unit / colblocks), cb = (uint32_t)(unit - (uint64_t)block * colblocks);
     const uint32_t BN = (uint32_t)hash.BN, BK = (uint32_t)hash.BK;
-    const uint32_t c0 = cb * 64, colA = c0 + lane, colB = colA + 32;
-    const uint32_t place = pb * 32 + lane;
-
-    uint32_t id = V, row = 0;
-    if (place < T_) {
-        if (sorted_id) {
-            id = sorted_id[place];
-            row = sorted_row[place];
-        } else {
-            const int64_t v = ids[place];
-            id = live_id(v, V, padding) ? (uint32_t)v : V;
-            row = place;
-        }
+    const uint32_t per_segment = (BN + 63) / 64, pn = cb / per_segment, in_segment = (cb - pn * per_segment) * 64;
+    const uint32_t end = min(BN, D - pn * BN);   // columns of the segment that exist
+    if (in_segment >= end) return;
+    const Places p = load_places(ids, padding, sorted_id, sorted_row, block, T_, V);
+    if (!p.live) return;
+    uint32_t dst = 0;
+    if (p.id < V) {
+        const uint32_t pk = p.id / BK, k_in = p.id - pk * BK;
+        dst = rz_tile_offset32(hash, hash32, pk, pn) + k_in * BN + in_segment;
     }
-    const uint32_t live = __ballot_sync(FULL, id < V);
-    if (!live) return;
-    const uint32_t pk = id / BK, k_in = id - pk * BK;
-    // where the words of this lane's place begin: of columns [c0, c0 + 32) and [c0 + 32, c0 + 64)
-    uint32_t dstA = 0, dstB = 0;
-    if (ALIGNED) {
-        const uint32_t pnA = c0 / BN, pnB = (c0 + 32) / BN;
-        if (id < V) {
-            const uint32_t offA = (uint32_t)rz_tile_offset(hash, pk, pnA);
-            const uint32_t offB = pnB == pnA || c0 + 32 >= D ? offA : (uint32_t)rz_tile_offset(hash, pk, pnB);
-            dstA = offA + k_in * BN + (c0 - pnA * BN);
-            dstB = offB + k_in * BN + (c0 + 32 - pnB * BN);
-        }
-    }
-    const uint32_t next = __shfl_down_sync(FULL, id, 1);
-    const uint32_t ends = __ballot_sync(FULL, lane == 31 || next != id);   // last place of each run
-
+    const bool has_a = in_segment + lane < end, has_b = in_segment + lane + 32 < end;
+    const T *src = dout + (size_t)pn * BN + in_segment + lane;
     float a = 0.f, b = 0.f;
     constexpr int U = 8;
 #pragma unroll 1
     for (int i0 = 0; i0 < 32; i0 += U) {
-        if (((live >> i0) & ((1u << U) - 1u)) == 0) continue;
+        const uint32_t live = p.live >> i0, ends = p.ends >> i0;
+        if ((live & ((1u << U) - 1u)) == 0) continue;
         float va[U], vb[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const uint32_t r = __shfl_sync(FULL, row, i0 + i);
-            const T *src = dout + (size_t)r * D;
+            const uint32_t r = __shfl_sync(FULL, p.row, i0 + i);
+            const T *at = src + (size_t)r * D;
             va[i] = vb[i] = 0.f;
-            if (!((live >> (i0 + i)) & 1u)) continue;
-            if (PACKED) {
-                if (c0 + 2 * lane < D) {
-                    const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(src + c0) + lane);
-                    va[i] = __uint_as_float(w << 16), vb[i] = __uint_as_float(w & 0xffff0000u);
-                }
-            } else {
-                if (colA < D) va[i] = to_f32<T>(src[colA]);
-                if (colB < D) vb[i] = to_f32<T>(src[colB]);
+            if ((live >> i) & 1u) {
+                if (has_a) va[i] = to_f32<T>(at[0]);
+                if (has_b) vb[i] = to_f32<T>(at[32]);
             }
         }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             a += va[i], b += vb[i];
-            if (!((ends >> (i0 + i)) & 1u)) continue;
-            if ((live >> (i0 + i)) & 1u) {
-                float x = a, y = b;
-                if (PACKED) {   // columns 2l, 2l + 1 -> l, 32 + l
-                    const uint32_t h = lane >> 1;
-                    const float xa = __shfl_sync(FULL, a, h), xb = __shfl_sync(FULL, b, h);
-                    const float ya = __shfl_sync(FULL, a, 16 + h), yb = __shfl_sync(FULL, b, 16 + h);
-                    x = (lane & 1) ? xb : xa, y = (lane & 1) ? yb : ya;
-                }
-                if (ALIGNED) {
-                    const uint32_t dA = __shfl_sync(FULL, dstA, i0 + i), dB = __shfl_sync(FULL, dstB, i0 + i);
-                    if (colA < D) atomicAdd(dH + dA + lane, x * alpha);
-                    if (colB < D) atomicAdd(dH + dB + lane, y * alpha);
-                } else {
-                    const uint32_t k = __shfl_sync(FULL, id, i0 + i), tk = k / BK, kin = k - tk * BK;
-                    if (colA < D) {
-                        const uint32_t pn = colA / BN;
-                        atomicAdd(dH + rz_tile_offset(hash, tk, pn) + (uint64_t)kin * BN + (colA - pn * BN), x * alpha);
-                    }
-                    if (colB < D) {
-                        const uint32_t pn = colB / BN;
-                        atomicAdd(dH + rz_tile_offset(hash, tk, pn) + (uint64_t)kin * BN + (colB - pn * BN), y * alpha);
-                    }
-                }
+            if (!((ends >> i) & 1u)) continue;
+            if ((live >> i) & 1u) {
+                float *word = dH + __shfl_sync(FULL, dst, i0 + i) + lane;
+                if (has_a) atomicAdd(word, a * alpha);
+                if (has_b) atomicAdd(word + 32, b * alpha);
             }
             a = b = 0.f;
         }
     }
 }
 
+// The shared-memory opt-in of a kernel, once per device.
+template <auto Kernel>
+int allow_smem(int bytes)
+{
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    int st = rz_record_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+    if (st) return st;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return RZ_OK;
+    st = rz_record_cuda(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "set max dynamic shared memory");
+    if (st) return st;
+    done.fetch_or(bit, std::memory_order_release);
+    return RZ_OK;
+}
+
 // Batches up to this length are not sorted: one launch less, and few repetitions to find.
 constexpr int64_t UNSORTED_TOKENS = 256;
 
+// Where a plan (the caller's buffer) has the sorted tokens; NULL for batches that are not sorted.
+struct SortedTokens {
+    uint32_t *id = nullptr, *row = nullptr;
+    SortedTokens(const rz_problem *pb, void *plan)
+    {
+        if (pb->M <= UNSORTED_TOKENS || !plan) return;
+        id = static_cast<uint32_t *>(plan);
+        row = id + pb->M;
+    }
+};
+
 template <int ITEMS>
-int launch_token_sort(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, int passes, uint32_t *sid, uint32_t *srow)
+int launch_token_sort(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const SortedTokens &sorted)
 {
     constexpr uint32_t CHUNK = CHUNK_THREADS * ITEMS;
     constexpr int SMEM = CHUNK * 4 + CHUNK_WARPS * 256 * 4 + CHUNK * 2;
     const uint32_t T = (uint32_t)c.pb->M;
-    int st = rz_record_cuda(cudaFuncSetAttribute(rz_token_sort_kernel<ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM),
-                            "set max dynamic shared memory");
+    int bits = 1;   // of the largest key, K
+    while (bits < 32 && (c.pb->K >> bits)) ++bits;
+    const int passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
+    const int st = allow_smem<rz_token_sort_kernel<ITEMS>>(SMEM);
     if (st) return st;
-    rz_token_sort_kernel<ITEMS><<<(T + CHUNK - 1) / CHUNK, CHUNK_THREADS, SMEM, c.stream>>>(ids, padding, T, (uint32_t)c.pb->K, passes,
-                                                                                         sid, srow);
+    rz_token_sort_kernel<ITEMS><<<(T + CHUNK - 1) / CHUNK, CHUNK_THREADS, SMEM, c.stream>>>(ids, padding, T, (uint32_t)c.pb->K, passes, width,
+                                                                                         sorted.id, sorted.row);
     rz_count_launch(1);
     return rz_record_cuda(cudaGetLastError(), "token sort launch");
 }
 
-template <typename T>
-int launch_embedding(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const float *hashed, void *out)
+int sort_tokens(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const SortedTokens &sorted)
+{
+    // the longest chunks whose sort (about 2.2 us for each 1024 tokens) the lookup hides, going by its bytes
+    const rz_problem *pb = c.pb;
+    const double lookup_us = (double)pb->M * (double)pb->N * (pb->io_dtype == RZ_BF16 ? 6.0 : 8.0) / 6e6;
+    if (pb->M > CHUNK_THREADS * 8 && lookup_us > 40.0) return launch_token_sort<16>(c, ids, padding, sorted);
+    if (pb->M > CHUNK_THREADS * 4 && lookup_us > 20.0) return launch_token_sort<8>(c, ids, padding, sorted);
+    if (pb->M > CHUNK_THREADS * 2) return launch_token_sort<4>(c, ids, padding, sorted);
+    return launch_token_sort<2>(c, ids, padding, sorted);
+}
+
+RzHash32 table_hash(const RzLaunchCtx &c)
 {
     const rz_problem *pb = c.pb;
-    const uint32_t D = (uint32_t)pb->N, nn = (D + pb->BN - 1) / (uint32_t)pb->BN;
-    const uint64_t total = (uint64_t)pb->M * nn;
+    return rz_hash32(c.hash, (uint64_t)(pb->K + pb->BK - 1) / pb->BK, (uint64_t)(pb->N + pb->BN - 1) / pb->BN);
+}
+
+template <typename T>
+int launch_embedding(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const float *hashed, void *out_, bool beside)
+{
+    const rz_problem *pb = c.pb;
+    T *out = static_cast<T *>(out_);
+    const uint32_t V = (uint32_t)pb->K, D = (uint32_t)pb->N, nn = (D + pb->BN - 1) / (uint32_t)pb->BN;
+    const RzHash32 hash32 = table_hash(c);
+    const bool aligned = (reinterpret_cast<uintptr_t>(out) & (2 * sizeof(T) - 1)) == 0;
+    const bool pieces = aligned && D % 64 == 0 && pb->BN % 64 == 0;
+    const uint64_t total = (uint64_t)pb->M * (pieces ? D / 64 : nn);
     // segments per warp: 32 (one hash evaluation for 32 of them) once that leaves enough warps, fewer for short batches
     uint32_t per_warp = 32;
     while (per_warp > 1 && total / per_warp < 148 * 32) per_warp >>= 1;
     const uint64_t warps = (total + per_warp - 1) / per_warp;
     uint64_t blocks = (warps + 7) / 8;
     if (blocks > 148 * 64) blocks = 148 * 64;
-    const bool pairs = D % 2 == 0 && pb->BN % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & (2 * sizeof(T) - 1)) == 0;
-    if (pairs)
-        rz_embedding_kernel<T, true><<<(unsigned)blocks, 256, 0, c.stream>>>(ids, padding, hashed, (T *)out, c.hash, total,
-                                                                            (uint32_t)pb->K, D, nn, per_warp, pb->alpha);
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = c.stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = beside ? 1 : 0;   // start while the token sort launched before runs
+    cudaError_t e;
+    if (pieces)
+        e = cudaLaunchKernelEx(&cfg, rz_embedding_pieces_kernel<T>, ids, padding, hashed, out, c.hash, hash32, total, V, D / 64, per_warp, pb->alpha);
+    else if (aligned && D % 2 == 0 && pb->BN % 2 == 0)
+        e = cudaLaunchKernelEx(&cfg, rz_embedding_kernel<T, true>, ids, padding, hashed, out, c.hash, hash32, total, V, D, nn, per_warp, pb->alpha);
     else
-        rz_embedding_kernel<T, false><<<(unsigned)blocks, 256, 0, c.stream>>>(ids, padding, hashed, (T *)out, c.hash, total,
-                                                                             (uint32_t)pb->K, D, nn, per_warp, pb->alpha);
+        e = cudaLaunchKernelEx(&cfg, rz_embedding_kernel<T, false>, ids, padding, hashed, out, c.hash, hash32, total, V, D, nn, per_warp, pb->alpha);
     rz_count_launch(1);
-    return rz_record_cuda(cudaGetLastError(), "embedding launch");
+    return rz_record_cuda(e, "embedding launch");
 }
 
 template <typename T>
-int launch_embedding_grad(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const uint32_t *sid, const uint32_t *srow,
-                          const void *dout, float *dH)
+int launch_embedding_grad(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const SortedTokens &sorted, const void *dout,
+                          float *dH)
 {
     const rz_problem *pb = c.pb;
-    const uint32_t D = (uint32_t)pb->N, M = (uint32_t)pb->M;
-    const uint32_t colblocks = (D + 63) / 64;
-    const uint64_t units = (uint64_t)((M + 31) / 32) * colblocks, blocks = (units + 7) / 8;
+    const uint32_t D = (uint32_t)pb->N, M = (uint32_t)pb->M, BN = (uint32_t)pb->BN;
+    const bool pairs = BN % 32 == 0 && D % 2 == 0 && (reinterpret_cast<uintptr_t>(dout) & (2 * sizeof(T) - 1)) == 0 &&
+                       (reinterpret_cast<uintptr_t>(dH) & 7u) == 0;
+    const RzHash32 hash32 = table_hash(c);
+    // two pieces of 64 columns a warp where that leaves eight warps per SM, one for short batches
+    const bool whole = BN % 64 == 0;
+    const uint32_t most = (M + 31) / 32;
+    const int pieces = pairs && D >= 128 && (uint64_t)most * ((D + 127) / 128) >= 148 * 8 ? 2 : 1;
+    const uint32_t colblocks = pairs ? (D + 64 * pieces - 1) / (64 * pieces) : (D + BN - 1) / BN * ((BN + 63) / 64);
+    const uint64_t units = (uint64_t)most * colblocks, blocks = (units + GRAD_THREADS / 32 - 1) / (GRAD_THREADS / 32);
     if (blocks > 0x7fffffffull) return RZ_ERR_SHAPE;
-    const bool aligned = pb->BN % 32 == 0;
-    const bool packed = sizeof(T) == 2 && D % 2 == 0 && (reinterpret_cast<uintptr_t>(dout) & 3u) == 0;
     auto run = [&](auto kernel) {
-        kernel<<<(unsigned)blocks, 256, 0, c.stream>>>(ids, padding, sid, srow, (const T *)dout, dH, c.hash, M, (uint32_t)pb->K, D,
+        kernel<<<(unsigned)blocks, GRAD_THREADS, 0, c.stream>>>(ids, padding, sorted.id, sorted.row, (const T *)dout, dH, c.hash, hash32, M, (uint32_t)pb->K, D,
                                                        colblocks, units, pb->alpha);
     };
-    constexpr bool P = sizeof(T) == 2;   // (the packed load exists for 2-byte elements only)
-    if (aligned && packed) run(rz_embedding_grad_kernel<T, true, P>);
-    else if (aligned) run(rz_embedding_grad_kernel<T, true, false>);
-    else if (packed) run(rz_embedding_grad_kernel<T, false, P>);
-    else run(rz_embedding_grad_kernel<T, false, false>);
+    if (pairs && pieces == 2) whole ? run(rz_embedding_grad_pairs_kernel<T, 2, true>) : run(rz_embedding_grad_pairs_kernel<T, 2, false>);
+    else if (pairs) whole ? run(rz_embedding_grad_pairs_kernel<T, 1, true>) : run(rz_embedding_grad_pairs_kernel<T, 1, false>);
+    else run(rz_embedding_grad_kernel<T>);
     rz_count_launch(1);
     return rz_record_cuda(cudaGetLastError(), "embedding gradient launch");
 }
@@ -517,43 +749,36 @@ int rz_rows_sort(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order
     uint32_t per = SORT_TILE;
     const uint32_t blocks = rows > 0 ? sort_blocks(rows, &per) : 1;
     uint32_t *hist = blocks > 1 ? static_cast<uint32_t *>(scratch) : nullptr;
+    int bits = 1;   // of the largest bin number, `bins`, plus one value more
+    while (((bins + 1) >> bits) != 0) ++bits;
     const int smem = (int)(sizeof(uint32_t) * (SORT_WARPS + 1) * (size_t)(bins + 1));
-    int st = rz_record_cuda(cudaFuncSetAttribute(rz_sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)(sizeof(uint32_t) * (SORT_WARPS + 1) * (SORT_MAX_BINS + 1))),
-                            "set max dynamic shared memory");
+    int st = allow_smem<rz_sort_place_kernel>((int)(sizeof(uint32_t) * (SORT_WARPS + 1) * (SORT_MAX_BINS + 1)));
     if (st) return st;
     if (hist) {
         rz_sort_count_kernel<<<blocks, SORT_THREADS, 0, stream>>>(keys, (uint32_t)rows, (uint32_t)bins, per, hist);
         rz_count_launch(1);
     }
-    rz_sort_place_kernel<<<blocks, SORT_THREADS, smem, stream>>>(keys, (uint32_t)rows, (uint32_t)bins, per, hist, order, offsets);
+    rz_sort_place_kernel<<<blocks, SORT_THREADS, smem, stream>>>(keys, (uint32_t)rows, (uint32_t)bins, per, bits, hist, order, offsets);
     rz_count_launch(1);
     return rz_record_cuda(cudaGetLastError(), "row sort launch");
 }
 
-int rz_rows_embedding(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const float *hashed, void *out)
+int rz_rows_embedding(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const float *hashed, void *out, void *plan)
 {
-    if (c.pb->io_dtype == RZ_BF16) return launch_embedding<__nv_bfloat16>(c, ids, padding, hashed, out);
-    return launch_embedding<float>(c, ids, padding, hashed, out);
-}
-
-size_t rz_rows_embedding_scratch(const rz_problem *pb) { return pb->M <= UNSORTED_TOKENS ? 0 : sizeof(uint32_t) * 2 * (size_t)pb->M; }
-
-int rz_rows_embedding_grad(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const void *dout, float *dH, void *scratch)
-{
-    const rz_problem *pb = c.pb;
-    uint32_t *sid = nullptr, *srow = nullptr;
-    if (pb->M > UNSORTED_TOKENS) {
-        sid = static_cast<uint32_t *>(scratch);
-        srow = sid + pb->M;
-        int bits = 1;   // of the largest key, V
-        while (bits < 32 && (pb->K >> bits)) ++bits;
-        const int passes = (bits + 7) / 8;
-        const int st = pb->M <= CHUNK_THREADS * 2   ? launch_token_sort<2>(c, ids, padding, passes, sid, srow)
-                       : pb->M <= CHUNK_THREADS * 4 ? launch_token_sort<4>(c, ids, padding, passes, sid, srow)
-                                                    : launch_token_sort<8>(c, ids, padding, passes, sid, srow);
+    const SortedTokens sorted(c.pb, plan);
+    if (sorted.id) {
+        const int st = sort_tokens(c, ids, padding, sorted);
         if (st) return st;
     }
-    if (pb->io_dtype == RZ_BF16) return launch_embedding_grad<__nv_bfloat16>(c, ids, padding, sid, srow, dout, dH);
-    return launch_embedding_grad<float>(c, ids, padding, sid, srow, dout, dH);
+    if (c.pb->io_dtype == RZ_BF16) return launch_embedding<__nv_bfloat16>(c, ids, padding, hashed, out, sorted.id != nullptr);
+    return launch_embedding<float>(c, ids, padding, hashed, out, sorted.id != nullptr);
+}
+
+size_t rz_rows_embedding_plan(const rz_problem *pb) { return pb->M <= UNSORTED_TOKENS ? 0 : sizeof(uint32_t) * 2 * (size_t)pb->M; }
+
+int rz_rows_embedding_grad(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const void *dout, float *dH, const void *plan)
+{
+    const SortedTokens sorted(c.pb, const_cast<void *>(plan));
+    if (c.pb->io_dtype == RZ_BF16) return launch_embedding_grad<__nv_bfloat16>(c, ids, padding, sorted, dout, dH);
+    return launch_embedding_grad<float>(c, ids, padding, sorted, dout, dH);
 }

@@ -17,6 +17,7 @@ Differences, all additive:
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -50,6 +51,18 @@ def make_problem(M, K, N, H, R, BLOCK_SIZE_K, BLOCK_SIZE_N, dtype, allow_tf32, i
         raise AssertionError("H must be larger than BLOCK_SIZE_K * BLOCK_SIZE_N")
     return _lib.make_problem(M, K, N, H, BLOCK_SIZE_K, BLOCK_SIZE_N, R, hash_mode, _lib.torch_io_dtype(dtype),
                              _precision(dtype, allow_tf32), init_factor, flags)
+
+
+# Filling an RzProblem costs several microseconds, which is what small problems are bound by; problems are never written to, so
+# calls with equal arguments may share one.
+_cached_problem = lru_cache(maxsize=256)(make_problem)
+
+
+def cached_problem(M, K, N, H, random_numbers, BLOCK_SIZE_K, BLOCK_SIZE_N, dtype, allow_tf32, init_factor, hash_mode, flags=0):
+    """make_problem from the random-number tensor of a layer."""
+    assert random_numbers.numel() == 8
+    return _cached_problem(M, K, N, H, tuple(random_numbers.tolist()), BLOCK_SIZE_K, BLOCK_SIZE_N, dtype, allow_tf32,
+                           float(init_factor), hash_mode, flags)
 
 
 def alloc_shadow(pb, hashed: torch.Tensor) -> Optional[torch.Tensor]:
@@ -97,7 +110,7 @@ def cached_shadow(pb, hashed_weight: torch.Tensor, hashed_f32: torch.Tensor, nby
         version, ptr = hashed_weight._version, hashed_weight.data_ptr()
     except RuntimeError:            # inference tensors keep no version counter: nothing to key a cache on
         return alloc_shadow(pb, hashed_f32)
-    stream = torch.cuda.current_stream(hashed_f32.device)
+    stream = _lib._stream(hashed_f32.device)
     if torch.cuda.is_current_stream_capturing():
         # a buffer from the graph's own memory pool, filled by a node of the graph; the eager cache is left alone
         shadow = torch.empty(nbytes, dtype=torch.uint8, device=hashed_f32.device)
@@ -106,16 +119,16 @@ def cached_shadow(pb, hashed_weight: torch.Tensor, hashed_f32: torch.Tensor, nby
     entry = cache.get(key)
     if entry is not None and entry["shadow"].numel() >= nbytes and entry["shadow"].device == hashed_f32.device:
         if entry["version"] == version and entry["ptr"] == ptr:
-            if entry["stream"] != stream.cuda_stream:
-                stream.wait_event(entry["filled"])    # the refresh ran on another stream
+            if entry["stream"] != stream:
+                torch.cuda.current_stream(hashed_f32.device).wait_event(entry["filled"])    # the refresh ran on another stream
             return entry["shadow"]
         shadow = entry["shadow"]                      # same buffer, new contents
     else:
         shadow = torch.empty(nbytes, dtype=torch.uint8, device=hashed_f32.device)
     _lib.shadow_refresh(pb, hashed_f32, shadow)
     filled = torch.cuda.Event()
-    filled.record(stream)
-    cache[key] = {"version": version, "ptr": ptr, "shadow": shadow, "stream": stream.cuda_stream, "filled": filled}
+    filled.record(torch.cuda.current_stream(hashed_f32.device))
+    cache[key] = {"version": version, "ptr": ptr, "shadow": shadow, "stream": stream, "filled": filled}
     return shadow
 
 

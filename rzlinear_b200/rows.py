@@ -12,7 +12,7 @@ def _index_view(t: torch.Tensor, what: str) -> torch.Tensor:
     """Contiguous int64 indices."""
     if t.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{what} must be int64 or int32, got {t.dtype}")
-    return t.to(torch.int64).contiguous()
+    return (t if t.dtype == torch.int64 else t.to(torch.int64)).contiguous()
 
 
 def sort_rows(keys: torch.Tensor, num_bins: int) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -82,8 +82,16 @@ CASES = [
     (2048, 70000, 64, 64, 128, 0, None, "even"),   # row shorter than a hash tile
     (2049, 300, 320, 128, 64, 1, 5, "one"),
     (8192, 4096, 128, 32, 64, 1, None, "text"),
-    (8193, 131072, 72, 64, 64, 0, 7, "outside"),   # ids of three sort passes, rows of no table entry
-    (30000, 65536, 40, 32, 64, 1, None, "text"),   # 17-bit sentinel key
+    (8193, 131072, 72, 64, 64, 0, 7, "outside"),   # rows of no table entry
+    (30000, 65536, 40, 32, 64, 1, None, "text"),
+    (4096, 60000, 4, 32, 4, 1, 9, "even"),         # one chunk, full
+    (12289, 3000, 8, 32, 8, 0, None, "text"),      # a chunk of one token
+    (100000, 40, 2, 4, 2, 0, None, "outside"),     # many chunks, most tokens of no row
+    (16385, 100000, 1024, 32, 64, 1, 5, "text"),   # the longest chunks, and one of one token
+    (6000, 5000, 512, 32, 64, 1, None, "text"),    # four pieces of 64 columns a warp
+    (6000, 5000, 330, 32, 32, 1, 8, "text"),       # the same, halves of a piece apart, a ragged last piece
+    (6000, 900, 450, 16, 96, 0, None, "one"),
+    (5000, 2**31 - 2**13, 64, 2048, 64, 0, None, "outside"),   # the largest ids
     (20000, 2, 50, 1, 50, 0, None, "even"),
 ]
 
@@ -108,7 +116,7 @@ def make_ids(kind, T, V, padding, rng):
 def test_embedding(rz, T, V, D, BK, BN, mode, padding, kind, dtype):
     rng = np.random.RandomState(T + V + D)
     R = numbers(T + D, mode)
-    H = max(V * D // 8, 2 * BK * BN) + 5
+    H = min(max(V * D // 8, 2 * BK * BN), 1 << 22) + 5
     ids = make_ids(kind, T, V, padding, rng)
     live = (ids >= 0) & (ids < V) & (ids != (padding % V if padding is not None else -1))
     words = words_of(ids, live, V, D, H, BK, BN, R, mode)
@@ -156,7 +164,7 @@ def test_embedding_row_is_the_linear_layers_weight_row(rz):
     emb = rz.RzEmbedding(V, D, hashed_weight=w)
     lin = rz.RzLinear(V, D, hashed_weight=w, bias=False)
     got = lin(torch.eye(V, device=DEV))
-    assert torch.allclose(got, emb(torch.arange(V, device=DEV)), rtol=0, atol=1e-6 * float(w.abs().max()))
+    assert torch.allclose(got, emb(torch.arange(V, device=DEV)), rtol=0, atol=1e-6 * float(w.detach().abs().max()))
 
 
 def test_embedding_types_and_views(rz):
@@ -183,6 +191,22 @@ def test_embedding_types_and_views(rz):
                  rz.RzEmbedding(V, D, hashed_weight=w)._random_numbers.tolist(), 1)).to(DEV)].view(50, 4, D).bfloat16())
     (dwb,) = torch.autograd.grad(out.float().sum(), wb)
     assert dwb.dtype == BF16
+
+
+def test_embedding_gradient_without_a_plan(rz, rzlib):
+    T, V, D, BK, BN, H = 5000, 300, 128, 32, 64, 9000
+    R = numbers(5, 1)
+    ids = torch.randint(0, V, (T,), device=DEV)
+    g = torch.ones(T, D, device=DEV)                                               # (sums of ones are exact in any order)
+    pb = rzlib.make_problem(T, V, D, H, BK, BN, R, 1, rzlib.F32, rzlib.PREC_FP32)
+    alone = torch.empty(H, device=DEV)
+    rzlib.embedding_backward(pb, ids, -1, g, alone)
+    plan, out, planned = rzlib.embedding_plan(pb, torch.device(DEV)), torch.empty(T, D, device=DEV), torch.empty(H, device=DEV)
+    rzlib.embedding_forward(pb, ids, -1, torch.randn(H, device=DEV), out, plan)
+    rzlib.embedding_backward(pb, ids, -1, g, planned, plan)
+    assert torch.equal(alone, planned)
+    rzlib.embedding_backward(rzlib.with_fields(pb, flags=rzlib.FLAG_ACCUMULATE_DH), ids, -1, g, planned, plan)
+    assert torch.equal(planned, 2 * alone)
 
 
 def test_embedding_empty_and_no_tokens(rz):

@@ -45,19 +45,20 @@ def test_embedding_refusals(rzlib):
     some = ctypes.c_void_p(1 << 20)
     pb = _pb(rzlib)
     ref = ctypes.byref
-    assert lib.rz_embedding_forward(ref(pb), None, -1, some, some, None) == -1
-    assert lib.rz_embedding_forward(ref(pb), some, -1, some, None, None) == -1
-    assert lib.rz_embedding_forward(ref(pb), ctypes.c_void_p((1 << 20) + 4), -1, some, some, None) == -5
-    assert lib.rz_embedding_forward(ref(_pb(rzlib, H=2048)), some, -1, some, some, None) == -3
-    assert lib.rz_embedding_forward(ref(_pb(rzlib, K=0)), some, -1, some, some, None) == -2
-    assert lib.rz_embedding_forward(ref(_pb(rzlib, io=1, prec=1)), some, -1, some, some, None) == -4
-    assert lib.rz_embedding_scratch_bytes(ref(_pb(rzlib, M=256))) == 0
+    def fwd(pb=pb, ids=some, h=some, out=some, plan=None, pbytes=0):
+        return lib.rz_embedding_forward(ref(pb), ids, -1, h, out, plan, pbytes, None)
+
+    assert fwd(ids=None) == -1 and fwd(h=None) == -1 and fwd(out=None) == -1
+    assert fwd(ids=ctypes.c_void_p((1 << 20) + 4)) == -5 and fwd(out=ctypes.c_void_p((1 << 20) + 2)) == -5
+    assert fwd(pb=_pb(rzlib, H=2048)) == -3 and fwd(pb=_pb(rzlib, K=0)) == -2 and fwd(pb=_pb(rzlib, io=1, prec=1)) == -4
+    assert lib.rz_embedding_plan_bytes(ref(_pb(rzlib, M=256))) == 0
     big = _pb(rzlib, M=257)
-    need = lib.rz_embedding_scratch_bytes(ref(big))
-    assert need == 257 * 8
-    assert lib.rz_embedding_backward(ref(big), some, -1, some, some, None, 0, None) == -1
+    need = lib.rz_embedding_plan_bytes(ref(big))
+    assert need == 257 * 8 and fwd(pb=big, plan=some, pbytes=need - 1) == -11
+    assert fwd(pb=big, plan=ctypes.c_void_p((1 << 20) + 2), pbytes=need) == -5
     assert lib.rz_embedding_backward(ref(big), some, -1, some, some, some, need - 1, None) == -11
     assert lib.rz_embedding_backward(ref(pb), some, -1, some, None, None, 0, None) == -1
+    assert lib.rz_embedding_backward(ref(pb), some, -1, None, some, None, 0, None) == -1
 
     layer = rz.RzEmbedding(1000, 64)
     assert layer._hashed_weight.shape == (4000,) and set(dict(layer.named_parameters())) == {"_hashed_weight"}
@@ -108,11 +109,13 @@ def test_grouped_refusals(rzlib):
     assert fwd(off=None) == -1 and fwd(x=None) == -1 and fwd(y=None) == -1 and fwd(c=None) == -1 and fwd(w=None) == -1
     assert fwd(cb=copies - 1) == -11 and fwd(wb=ws - 1) == -11
     assert fwd(x=odd) == -5 and fwd(y=odd) == -5 and fwd(w=odd) == -5 and fwd(off=ctypes.c_void_p((1 << 20) + 2)) == -5
-    assert lib.rz_grouped_backward_weight(ref(pb), 4, some, some, some, None, some, ws, None) == -1
-    assert lib.rz_grouped_backward_weight(ref(pb), 4, some, some, some, some, some, ws - 1, None) == -11
-    assert lib.rz_grouped_backward_input(ref(pb), 4, some, None, some, some, copies, some, some, ws, None) == -1
-    assert lib.rz_grouped_grad_prepare(ref(pb), 4, some, some, None, None, None, some, ws, None) == -1
-    assert lib.rz_grouped_grad_prepare(ref(pb), 4, some, some, some, None, some, some, ws, None) == -1   # a mask, nowhere to write
+
+    def bwd(x=some, dy=some, y=None, h=some, c=some, dym=None, db=None, dx=some, dh=some, w=some, wb=ws):
+        return lib.rz_grouped_backward(ref(pb), 4, some, x, dy, y, h, c, copies, dym, db, dx, dh, w, wb, None)
+
+    assert bwd(dy=None) == -1 and bwd(x=None) == -1 and bwd(c=None) == -1 and bwd(dx=None, dh=None) == -1 and bwd(w=None) == -1
+    assert bwd(y=some) == -1                                                            # a mask, and nowhere to put the masked gradient
+    assert bwd(wb=ws - 1) == -11 and bwd(dy=odd) == -5 and bwd(x=odd) == -5 and bwd(dx=odd) == -5 and bwd(y=some, dym=odd) == -5
 
     layer = rz.RzGroupedLinear(4, 128, 64)
     assert layer._hashed_weight.shape == (2048,) and layer._bias.shape == (4, 64)
