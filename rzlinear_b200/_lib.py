@@ -324,9 +324,9 @@ def embedding_backward(pb, ids, padding_idx, dout, dh, plan=None) -> None:
 def grouped_sizes(pb, groups: int):
     """(bytes of shifted copies, bytes of workspace) of a grouped problem; remembered on the problem, which is never written to."""
     known = getattr(pb, "_grouped_sizes", None)
-    if known is None or known[0] != groups:
+    if known is None or known[0] != (groups, _env_reads):
         lib = load()
-        known = (groups, int(lib.rz_grouped_copies_bytes(ctypes.byref(pb))),
+        known = ((groups, _env_reads), int(lib.rz_grouped_copies_bytes(ctypes.byref(pb))),
                  max(256, int(lib.rz_grouped_workspace_bytes(ctypes.byref(pb), groups))))
         pb._grouped_sizes = known
     return known[1:]
@@ -382,9 +382,14 @@ def launch_count() -> int:
     return int(load().rz_launch_count())
 
 
+_env_reads = 0
+
+
 def reload_env() -> None:
     """Make the library read its RZ_TC_* bring-up knobs from the environment again."""
+    global _env_reads
     load().rz_reload_env()
+    _env_reads += 1          # sizes remembered on problems may have been others
 
 
 NOALLOC_SCRATCH_BYTES = 16 << 20

@@ -19,7 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "librzlinear_b200.so")
 SOURCES = ["rz_abi.cu", "rz_simt.cu", "rz_tc.cu", "rz_noalloc.cu", "rz_elementwise.cu", "rz_rows.cu",
            "rz_grouped.cu", "rz_tc_grouped.cu"]
-HEADERS = ["rz_common.h", "rz_hash.h", "rz_ptx.cuh", "rz_tc_kernel.cuh", "rz_tc_host.h", os.path.join("..", "..", "include", "rzlinear_b200.h")]
+HEADERS = ["rz_common.h", "rz_hash.h", "rz_ptx.cuh", "rz_tc_kernel.cuh", "rz_tc_rows.cuh", "rz_tc_host.h", os.path.join("..", "..", "include", "rzlinear_b200.h")]
 
 
 def _nvcc() -> str:

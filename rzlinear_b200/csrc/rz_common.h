@@ -105,8 +105,9 @@ int rz_simt_grouped_backward_weight(const RzLaunchCtx &c, const RzGroupPieces &p
 
 // tensor-core launches of a grouped operation (rz_tc_grouped.cu)
 struct RzTcGroupPlan {
-    int ctas, rb, nc, ew;   // block shape
+    int ctas, rb, nc, ew;   // block shape (bf16 products: nc = most rows of a block)
     uint32_t step;          // most rows of a piece
+    bool even;              // a group's pieces are equal
 };
 RzTcGroupPlan rz_tc_grouped_plan(const rz_problem *pb, int groups, int op);
 int rz_tc_grouped_forward(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *X, const void *copies,

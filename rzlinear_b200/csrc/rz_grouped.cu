@@ -16,7 +16,8 @@ constexpr int PLAN_THREADS = 1024;
 struct PlanList {
     uint32_t *header;       // [0] = pieces
     uint4 *entries;
-    uint32_t step;
+    uint32_t step;          // most rows of a piece
+    uint32_t even;          // != 0: a group's pieces are equal, in multiples of 16 rows; else all but the last have `step` rows
 };
 
 constexpr int MAX_LISTS = 3;
@@ -105,8 +106,13 @@ rz_group_plan_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
                 if (first[mid] <= i) lo = mid;
                 else hi = mid;
             }
-            const uint32_t row = bound[lo] + (i - first[lo]) * list.step;
-            list.entries[i] = make_uint4(lo, row, min(row + list.step, bound[lo + 1]), 0u);
+            uint32_t rows = list.step;
+            if (list.even) {
+                const uint32_t n = bound[lo + 1] - bound[lo], count = (n + list.step - 1) / list.step;
+                rows = ((n + count - 1) / count + 15) / 16 * 16;   // (<= step, a multiple of 16; the last piece is not empty)
+            }
+            const uint32_t row = bound[lo] + (i - first[lo]) * rows;
+            list.entries[i] = make_uint4(lo, row, min(row + rows, bound[lo + 1]), 0u);
         }
         if (!alone || blockIdx.x) return;
     }
@@ -162,10 +168,18 @@ size_t pieces_bytes(const rz_problem *pb, int groups, uint32_t step)
     return (256 + sizeof(uint4) * (size_t)most_pieces(pb, groups, step) + 255) / 256 * 256;
 }
 
-uint32_t step_of(const rz_problem *pb, int groups, int op, bool tc)
+struct Step {
+    uint32_t rows;
+    bool even;
+};
+
+Step step_of(const rz_problem *pb, int groups, int op, bool tc)
 {
-    if (tc) return rz_tc_grouped_plan(pb, groups, op).step;
-    return op == RZ_OP_BACKWARD_WEIGHT ? SIMT_CHUNK : SIMT_ROWS;
+    if (tc) {
+        const RzTcGroupPlan plan = rz_tc_grouped_plan(pb, groups, op);
+        return Step{plan.step, plan.even};
+    }
+    return Step{op == RZ_OP_BACKWARD_WEIGHT ? SIMT_CHUNK : SIMT_ROWS, false};
 }
 
 // A plan under construction: lists are added one behind the other in the workspace, then one launch writes them all.
@@ -182,11 +196,13 @@ struct Plan {
         args.offsets = offsets;
         args.groups = (uint32_t)groups_, args.M = (uint32_t)c_.pb->M;
     }
-    RzGroupPieces add(uint32_t step)
+    RzGroupPieces add(const Step &s)
     {
+        const uint32_t step = s.rows;
         RzGroupPieces pieces;
         PlanList &l = args.list[args.lists++];
         l.step = step;
+        l.even = s.even;
         l.header = reinterpret_cast<uint32_t *>(ws + used);
         l.entries = reinterpret_cast<uint4 *>(ws + used + 256);
         used += pieces_bytes(c.pb, groups, step);
@@ -285,9 +301,9 @@ uint64_t element_bytes(const rz_problem *pb) { return pb->io_dtype == RZ_BF16 ? 
 size_t rz_grouped_workspace(const rz_problem *pb, int groups, bool tc)
 {
     // the backward's three lists and the weight gradient's maps, or the forward's list
-    const size_t forward = pieces_bytes(pb, groups, step_of(pb, groups, RZ_OP_FORWARD, tc));
-    const size_t backward = pieces_bytes(pb, groups, PREPARE_ROWS) + pieces_bytes(pb, groups, step_of(pb, groups, RZ_OP_BACKWARD_INPUT, tc)) +
-                            pieces_bytes(pb, groups, step_of(pb, groups, RZ_OP_BACKWARD_WEIGHT, tc)) +
+    const size_t forward = pieces_bytes(pb, groups, step_of(pb, groups, RZ_OP_FORWARD, tc).rows);
+    const size_t backward = pieces_bytes(pb, groups, PREPARE_ROWS) + pieces_bytes(pb, groups, step_of(pb, groups, RZ_OP_BACKWARD_INPUT, tc).rows) +
+                            pieces_bytes(pb, groups, step_of(pb, groups, RZ_OP_BACKWARD_WEIGHT, tc).rows) +
                             (tc ? 2 * sizeof(CUtensorMap) * (size_t)groups : 0);
     return forward > backward ? forward : backward;
 }
@@ -314,7 +330,7 @@ int rz_grouped_run_backward(const RzLaunchCtx &c, int groups, const int32_t *off
     Plan plan(c, groups, offsets, ws);
     RzGroupPieces rows, blocks, chunks;
     int st;
-    if (prepare) rows = plan.add(PREPARE_ROWS);
+    if (prepare) rows = plan.add(Step{PREPARE_ROWS, false});
     if (dX) {
         blocks = plan.add(step_of(pb, groups, RZ_OP_BACKWARD_INPUT, tc));
         plan.clear(dX, element_bytes(pb) * (uint64_t)pb->K);

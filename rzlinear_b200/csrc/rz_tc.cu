@@ -305,7 +305,7 @@ struct MapCache {
 
 namespace rztc {
 
-int encode(CUtensorMap *map, bool tf32, bool mn_major, void *base, int rank, const uint64_t *dims,
+int encode(CUtensorMap *map, bool tf32, int mn_major, void *base, int rank, const uint64_t *dims,
            const uint64_t *strides_bytes, const uint32_t *box)
 {
     static thread_local MapCache cache;
@@ -340,7 +340,9 @@ int encode(CUtensorMap *map, bool tf32, bool mn_major, void *base, int rank, con
     for (int i = 0; i + 1 < rank; ++i) gstr[i] = strides_bytes[i];
     CUresult r = fn(map, tf32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, base,
                     gdim, gstr, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    (tf32 && mn_major) ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+                    mn_major == PLAIN_LAYOUT ? CU_TENSOR_MAP_SWIZZLE_NONE
+                    : (tf32 && mn_major)     ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
+                                             : CU_TENSOR_MAP_SWIZZLE_128B,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         char msg[96];
@@ -780,7 +782,7 @@ int forced_shape()
 }
 
 // 2-D map over a row-major matrix [rows][cols] of the operand type
-int map_matrix(CUtensorMap *map, bool tf32, bool mn_major, const void *base, uint64_t rows, uint64_t cols,
+int map_matrix(CUtensorMap *map, bool tf32, int mn_major, const void *base, uint64_t rows, uint64_t cols,
                uint32_t box_cols, uint32_t box_rows)
 {
     const int es = tf32 ? 4 : 2;

@@ -1,11 +1,12 @@
-// Tensor-core launches of products grouped by row: block shapes and descriptors for the GROUPED instantiations of
-// rz_tc_kernel.cuh.  The number of blocks is known on the device only, so every launch fills the machine (one CTA or CTA pair per
+// Tensor-core launches of products grouped by row: bf16 products run rz_tc_rows.cuh, their weight gradient and all fp32 operations
+// the GROUPED instantiations of rz_tc_kernel.cuh.  The number of blocks is known on the device only, so every launch fills the machine (one CTA or CTA pair per
 // SM or pair of SMs) and the kernel deals the planned pieces' blocks out round robin.
 #include <atomic>
 #include <cstring>
 
 #include "rz_tc_host.h"
 #include "rz_tc_kernel.cuh"
+#include "rz_tc_rows.cuh"
 
 using namespace rztc;
 
@@ -16,6 +17,160 @@ int usable_sms(const rz_problem *pb)
     const int n = num_sms() - (pb->sm_reserve > 0 ? pb->sm_reserve : 0);
     return n < 2 ? 2 : n;
 }
+
+// Per kernel variant and device, once: the shared-memory opt-in, and how many blocks (pairs) can be resident.
+template <auto Kernel, int CTAS>
+int resident(const rz_problem *pb, int threads, int smem, int *slots)
+{
+    static std::atomic<int> ready[64];   // 0 = not set up, else resident blocks / pairs + 1
+    int dev = 0;
+    int st = rz_record_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+    if (st) return st;
+    const bool cacheable = dev >= 0 && dev < 64;
+    const int known = cacheable ? ready[dev].load(std::memory_order_acquire) : 0;
+    *slots = num_sms() / CTAS;
+    if (known) {
+        *slots = known - 1;
+    } else {
+        st = rz_record_cuda(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "set max dynamic shared memory");
+        if (st) return st;
+        if (CTAS == 2) {
+            cudaLaunchConfig_t cfg;
+            cudaLaunchAttribute attr[1];
+            memset(&cfg, 0, sizeof(cfg));
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+            cfg.blockDim = dim3(threads, 1, 1);
+            cfg.dynamicSmemBytes = smem;
+            cfg.gridDim = dim3(2 * (unsigned)*slots, 1, 1);
+            cfg.attrs = attr, cfg.numAttrs = 1;
+            int clusters = 0;
+            if (cudaOccupancyMaxActiveClusters(&clusters, Kernel, &cfg) == cudaSuccess && clusters > 0 && clusters < *slots) *slots = clusters;
+            (void)cudaGetLastError();
+        }
+        if (cacheable) ready[dev].store(*slots + 1, std::memory_order_release);
+    }
+    if (pb->sm_reserve > 0) {   // leave SMs idle for whatever the caller runs beside this kernel
+        *slots -= (pb->sm_reserve + CTAS - 1) / CTAS;
+        if (*slots < 1) *slots = 1;
+    }
+    return RZ_OK;
+}
+
+// One CTA (pair) per slot, or per block where `most` says that there are fewer.
+template <int CTAS, typename Kernel, typename... Args>
+int launch_persistent(Kernel kernel, int threads, int smem, int slots, uint64_t most, cudaStream_t stream, const Args &...args)
+{
+    if (most >= 0x80000000ull) return RZ_ERR_SHAPE;   // block numbers are 32-bit words
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[1];
+    memset(&cfg, 0, sizeof(cfg));
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CTAS, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.gridDim = dim3((unsigned)(most < (uint64_t)slots ? most : (uint64_t)slots) * CTAS, 1, 1);
+    cfg.attrs = attr, cfg.numAttrs = CTAS == 2 ? 1 : 0;
+    const int st = rz_record_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), "grouped tcgen05 kernel launch");
+    rz_count_launch(1);
+    if (st) return st;
+    return rz_record_cuda(cudaGetLastError(), "grouped tcgen05 kernel launch");
+}
+
+// ---- bf16 products (rz_tc_rows.cuh) -----------------------------------------------------------------------------------------
+
+// weight rows per box: whole boxes per hash tile
+uint32_t rows_box(const rz_problem *pb, int op)
+{
+    if (pb->BK < 64) return 32;   // (BK is 32, 64 or a multiple of 64)
+    return op == RZ_OP_BACKWARD_INPUT && pb->BK % 128 == 0 ? 128 : 64;
+}
+
+template <int OP, int CTAS, int RB, int NMAX>
+int launch_rows(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *rows, const void *copies, const float *bias, void *out)
+{
+    const rz_problem *pb = c.pb;
+    constexpr int op = OP == ROWS_FWD ? RZ_OP_FORWARD : RZ_OP_BACKWARD_INPUT;
+    const int64_t depth = OP == ROWS_FWD ? pb->K : pb->N, cols = OP == ROWS_FWD ? pb->N : pb->K;
+    TcRowsParams p;
+    memset(&p, 0, sizeof(p));
+    p.hash = c.hash;
+    p.header = pieces.header, p.entries = pieces.entries, p.group_tiles = pieces.group_tiles;
+    p.cols = (uint32_t)cols;
+    p.tiles_c = (uint32_t)((cols + 128 * CTAS * RB - 1) / (128 * CTAS * RB));
+    p.nchunks = (uint32_t)((depth + 63) / 64);
+    p.br = rows_box(pb, op);
+    p.kparts = 64 / (p.br < 64 ? p.br : 64);
+    p.group_pieces = 8;
+    p.alpha = pb->alpha;
+    p.relu = OP == ROWS_FWD && (pb->flags & RZ_FLAG_RELU) ? 1 : 0;
+    p.bias = bias;
+    p.out = static_cast<__nv_bfloat16 *>(out);
+    int st = rz_wait_context(&p.wait, 2000000000ll);   // also refuses to launch behind a kernel whose wait gave up
+    if (st) return st;
+    CUtensorMap mapW, mapR, mapRAll, mapC;
+    st = map_shadow(&mapW, pb, OP == ROWS_FWD, copies, p.br);
+    if (st) return st;
+    st = map_matrix(&mapR, false, 0, rows, pb->M, depth, 64, 16);
+    if (st) return st;
+    st = map_matrix(&mapRAll, false, 0, rows, pb->M, depth, 64, NMAX / CTAS);
+    if (st) return st;
+    st = map_matrix(&mapC, false, PLAIN_LAYOUT, out, pb->M, cols, 32, 32);
+    if (st) return st;
+    constexpr int SMEM = rows_smem_total(CTAS, RB, NMAX), THREADS = 64 + 128 * RB;
+    static_assert(SMEM <= ROWS_SMEM_LIMIT, "shared memory budget");
+    int slots = 0;
+    st = resident<rz_tc_rows_kernel<OP, CTAS, RB, NMAX>, CTAS>(pb, THREADS, SMEM, &slots);
+    if (st) return st;
+    return launch_persistent<CTAS>(rz_tc_rows_kernel<OP, CTAS, RB, NMAX>, THREADS, SMEM, slots, (uint64_t)pieces.most * p.tiles_c, c.stream, mapW,
+                                   mapR, mapRAll, mapC, p);
+}
+
+template <int OP>
+int launch_rows_any(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *rows, const void *copies,
+                    const float *bias, void *out)
+{
+    if (plan.rb == 2) return launch_rows<OP, 2, 2, 256>(c, pieces, rows, copies, bias, out);
+    if (plan.ctas == 2) return launch_rows<OP, 2, 1, 256>(c, pieces, rows, copies, bias, out);
+    if (plan.nc == 256) return launch_rows<OP, 1, 1, 256>(c, pieces, rows, copies, bias, out);
+    if (plan.nc == 64) return launch_rows<OP, 1, 1, 64>(c, pieces, rows, copies, bias, out);
+    return launch_rows<OP, 1, 1, 32>(c, pieces, rows, copies, bias, out);
+}
+
+// Block shape of a bf16 product by an estimate of its time: waves of blocks over the SMs, times a block's stages at the slower of
+// fetching its operands (about 50 bytes a clock and SM) and multiplying them (8192 flops).
+RzTcGroupPlan rows_plan(const rz_problem *pb, int groups, int op)
+{
+    static const struct {
+        int ctas, rb, nmax;
+    } shapes[] = {{2, 2, 256}, {2, 1, 256}, {1, 1, 256}, {1, 1, 64}, {1, 1, 32}};
+    const double used = (double)(pb->M < groups ? pb->M : groups), mean = (double)pb->M / used;
+    const int64_t cols = op == RZ_OP_FORWARD ? pb->N : pb->K;
+    const double stages = (double)(((op == RZ_OP_FORWARD ? pb->K : pb->N) + 63) / 64);
+    const int sms = usable_sms(pb), forced = forced_shape();
+    RzTcGroupPlan best = {};
+    double best_time = -1.0;
+    for (int i = 0; i < 5; ++i) {
+        const auto &s = shapes[i];
+        const double pieces = (double)(int64_t)((mean + s.nmax - 1) / s.nmax), rows = mean / pieces;
+        const double width = (double)((int64_t)((rows + 16 * s.ctas - 1) / (16 * s.ctas)) * 16 * s.ctas);
+        const double fetch = (s.rb * 16384.0 + width / s.ctas * 128.0) / 50.0, multiply = 2.0 * width * s.rb;
+        // a block's clocks; two row blocks do not overlap their epilogue with the next block
+        const double block = stages * (fetch > multiply ? fetch : multiply) + (s.rb == 2 ? 5000.0 : 1500.0);
+        const double items = used * pieces * (double)((cols + 128 * s.ctas * s.rb - 1) / (128 * s.ctas * s.rb));
+        double waves = items * s.ctas / sms;
+        waves = waves < 1.0 ? 1.0 : waves + 0.5;               // half a wave is lost at the end
+        const double time = waves * block;
+        if (best_time < 0.0 || time < best_time || i == forced) {
+            best_time = i == forced ? 0.0 : time;
+            best.ctas = s.ctas, best.rb = s.rb, best.nc = s.nmax, best.ew = 1, best.step = (uint32_t)s.nmax, best.even = true;
+        }
+    }
+    return best;
+}
+
+// ---- GROUPED instantiations of rz_tc_kernel.cuh -------------------------------------------------------------------------------
 
 template <int OP, bool TF32, int CTAS, int RB, int SPLIT, int NC, int EW = 1>
 int launch(const RzLaunchCtx &c, const CUtensorMap &mapA, const CUtensorMap &mapB, const CUtensorMap &mapC, TcGroupParams &p,
@@ -56,76 +211,38 @@ int launch(const RzLaunchCtx &c, const CUtensorMap &mapA, const CUtensorMap &map
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a_major << 15) | (b_major << 16) | ((uint32_t)(NC >> 3) << 17) |
               ((uint32_t)(PAIR_R >> 4) << 24);
 
-    auto kern = rz_tc_kernel<OP, TF32, CTAS, RB, SPLIT, NC, EW, 1>;
-    // per kernel variant and device, once: the shared-memory opt-in and how many clusters fit the device
-    static std::atomic<int> ready[64];   // 0 = not set up, else resident blocks / pairs + 1
-    int dev = 0;
-    st = rz_record_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+    constexpr int THREADS = num_threads(RB, SPLIT, EW);
+    int slots = 0;
+    st = resident<rz_tc_kernel<OP, TF32, CTAS, RB, SPLIT, NC, EW, 1>, CTAS>(pb, THREADS, SMEM_TOTAL, &slots);
     if (st) return st;
-    const bool cacheable = dev >= 0 && dev < 64;
-    const int known = cacheable ? ready[dev].load(std::memory_order_acquire) : 0;
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cudaLaunchAttribute attr[1];
-    cfg.blockDim = dim3(num_threads(RB, SPLIT, EW), 1, 1);
-    cfg.dynamicSmemBytes = SMEM_TOTAL;
-    cfg.stream = c.stream;
-    int slots = num_sms() / CTAS;
-    if (CTAS == 2) {
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 2;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        cfg.gridDim = dim3(2 * (unsigned)slots, 1, 1);
-    }
-    if (known) {
-        slots = known - 1;
-    } else {
-        st = rz_record_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL),
-                            "set max dynamic shared memory");
-        if (st) return st;
-        if (CTAS == 2) {
-            int clusters = 0;
-            if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0 && clusters < slots)
-                slots = clusters;
-            (void)cudaGetLastError();
-        }
-        if (cacheable) ready[dev].store(slots + 1, std::memory_order_release);
-    }
-    if (pb->sm_reserve > 0) {
-        slots -= (pb->sm_reserve + CTAS - 1) / CTAS;
-        if (slots < 1) slots = 1;
-    }
     const uint64_t most = (uint64_t)pieces.most * p.tiles_c * (OP == OP_DW ? p.tiles_r : 1);
-    if (most >= 0x80000000ull) return RZ_ERR_SHAPE;   // block numbers are 32-bit words
-    cfg.gridDim = dim3((unsigned)(most < (uint64_t)slots ? most : (uint64_t)slots) * CTAS, 1, 1);
-    st = rz_record_cuda(cudaLaunchKernelEx(&cfg, kern, mapA, mapB, mapC, p), "grouped tcgen05 kernel launch");
-    rz_count_launch(1);
-    if (st) return st;
-    return rz_record_cuda(cudaGetLastError(), "grouped tcgen05 kernel launch");
+    return launch_persistent<CTAS>(rz_tc_kernel<OP, TF32, CTAS, RB, SPLIT, NC, EW, 1>, THREADS, SMEM_TOTAL, slots, most, c.stream, mapA, mapB, mapC,
+                                   p);
 }
 
 template <int OP>
 int launch_any(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const CUtensorMap &mapA, const CUtensorMap &mapB, const CUtensorMap &mapC,
                TcGroupParams &p, const RzGroupPieces &pieces)
 {
-    const bool tf32 = c.pb->precision == RZ_PREC_TF32;
     if (c.pb->precision == RZ_PREC_FP32) {
         if (plan.nc == 128) return launch<OP, true, 1, 1, 1, 128>(c, mapA, mapB, mapC, p, pieces);
         return launch<OP, true, 1, 1, 1, 64>(c, mapA, mapB, mapC, p, pieces);
     }
     constexpr int W1 = OP == OP_DW ? 4 : 1, W2 = OP == OP_DW ? 2 : 1;   // epilogue warps per TMEM lane quarter and row block
-    if (plan.rb == 2)
-        return tf32 ? launch<OP, true, 2, 2, 0, 256, W2>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 2, 2, 0, 256, W2>(c, mapA, mapB, mapC, p, pieces);
-    if (plan.ctas == 2)
-        return tf32 ? launch<OP, true, 2, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 2, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces);
-    if (plan.nc == 256)
-        return tf32 ? launch<OP, true, 1, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 1, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces);
-    if (plan.nc == 128)
-        return tf32 ? launch<OP, true, 1, 1, 0, 128, W1>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 1, 1, 0, 128, W1>(c, mapA, mapB, mapC, p, pieces);
-    return tf32 ? launch<OP, true, 1, 1, 0, 64, W1>(c, mapA, mapB, mapC, p, pieces) : launch<OP, false, 1, 1, 0, 64, W1>(c, mapA, mapB, mapC, p, pieces);
+    if constexpr (OP == OP_DW) {
+        if (c.pb->precision == RZ_PREC_BF16) {
+            if (plan.rb == 2) return launch<OP, false, 2, 2, 0, 256, W2>(c, mapA, mapB, mapC, p, pieces);
+            if (plan.ctas == 2) return launch<OP, false, 2, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces);
+            if (plan.nc == 256) return launch<OP, false, 1, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces);
+            if (plan.nc == 128) return launch<OP, false, 1, 1, 0, 128, W1>(c, mapA, mapB, mapC, p, pieces);
+            return launch<OP, false, 1, 1, 0, 64, W1>(c, mapA, mapB, mapC, p, pieces);
+        }
+    }
+    if (plan.rb == 2) return launch<OP, true, 2, 2, 0, 256, W2>(c, mapA, mapB, mapC, p, pieces);
+    if (plan.ctas == 2) return launch<OP, true, 2, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces);
+    if (plan.nc == 256) return launch<OP, true, 1, 1, 0, 256, W1>(c, mapA, mapB, mapC, p, pieces);
+    if (plan.nc == 128) return launch<OP, true, 1, 1, 0, 128, W1>(c, mapA, mapB, mapC, p, pieces);
+    return launch<OP, true, 1, 1, 0, 64, W1>(c, mapA, mapB, mapC, p, pieces);
 }
 
 }  // namespace
@@ -135,6 +252,7 @@ int launch_any(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const CUtensorMa
 // but not how the rows are spread: it reckons with even groups, each with half a ragged block at its end.
 RzTcGroupPlan rz_tc_grouped_plan(const rz_problem *pb, int groups, int op)
 {
+    if (pb->precision == RZ_PREC_BF16 && op != RZ_OP_BACKWARD_WEIGHT) return rows_plan(pb, groups, op);
     static const struct {
         int ctas, rb, nc;
         double speed;
@@ -144,7 +262,7 @@ RzTcGroupPlan rz_tc_grouped_plan(const rz_problem *pb, int groups, int op)
     const double used = (double)(pb->M < groups ? pb->M : groups), mean = (double)pb->M / used;
     const int64_t cols = op == RZ_OP_FORWARD ? pb->N : pb->K;
     const int sms = usable_sms(pb);
-    RzTcGroupPlan best = {1, 1, 64, 4, 128};
+    RzTcGroupPlan best = {1, 1, 64, 4, 128, false};
     double best_time = -1.0;
     const int forced = forced_shape();
     for (int i = 0; i < 5; ++i) {
@@ -187,18 +305,18 @@ int rz_tc_grouped_forward(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const
                           const float *bias, void *Y)
 {
     const rz_problem *pb = c.pb;
-    const bool tf32 = pb->precision != RZ_PREC_BF16;
+    if (pb->precision == RZ_PREC_BF16) return launch_rows_any<ROWS_FWD>(c, plan, pieces, X, copies, bias, Y);
     const Geometry g = geometry(pb);
     TcGroupParams p;
     memset(&p, 0, sizeof(p));
     p.bias = bias;
     p.out = Y;
     CUtensorMap mapA, mapB, mapC;
-    int st = map_matrix(&mapA, tf32, false, X, pb->M, pb->K, g.epr, TILE_R);
+    int st = map_matrix(&mapA, true, 0, X, pb->M, pb->K, g.epr, TILE_R);
     if (st) return st;
     st = map_shadow(&mapB, pb, true, copies, pb->BK < g.epr ? pb->BK : g.epr);
     if (st) return st;
-    st = map_matrix(&mapC, tf32, false, Y, pb->M, pb->N, g.epr, 32);
+    st = map_matrix(&mapC, true, 0, Y, pb->M, pb->N, g.epr, 32);
     if (st) return st;
     return launch_any<OP_FWD>(c, plan, mapA, mapB, mapC, p, pieces);
 }
@@ -207,18 +325,18 @@ int rz_tc_grouped_backward_input(const RzLaunchCtx &c, const RzTcGroupPlan &plan
                                  const void *copies, void *dX)
 {
     const rz_problem *pb = c.pb;
-    const bool tf32 = pb->precision != RZ_PREC_BF16;
+    if (pb->precision == RZ_PREC_BF16) return launch_rows_any<ROWS_DX>(c, plan, pieces, dY, copies, nullptr, dX);
     const Geometry g = geometry(pb);
     TcGroupParams p;
     memset(&p, 0, sizeof(p));
     p.out = dX;
     CUtensorMap mapA, mapB, mapC;
-    int st = map_matrix(&mapA, tf32, false, dY, pb->M, pb->N, g.epr, TILE_R);
+    int st = map_matrix(&mapA, true, 0, dY, pb->M, pb->N, g.epr, TILE_R);
     if (st) return st;
     const uint32_t bcols = (uint32_t)(plan.nc / plan.ctas);
     st = map_shadow(&mapB, pb, false, copies, (uint32_t)pb->BK < bcols ? (uint32_t)pb->BK : bcols);
     if (st) return st;
-    st = map_matrix(&mapC, tf32, false, dX, pb->M, pb->K, g.epr, 32);
+    st = map_matrix(&mapC, true, 0, dX, pb->M, pb->K, g.epr, 32);
     if (st) return st;
     return launch_any<OP_DX>(c, plan, mapA, mapB, mapC, p, pieces);
 }

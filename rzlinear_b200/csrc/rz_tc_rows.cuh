@@ -1,0 +1,367 @@
+// Tensor-core kernel of products grouped by row, bf16: Y[r,:] = X[r,:] . W_g and dX[r,:] = dY[r,:] . W_g^T for the rows r of group g.
+//
+// The block is computed TRANSPOSED: the weight's columns (FWD; its rows for DX) are the MMA's M, the group's rows its N.  M comes in
+// blocks of 128 a CTA and weights are that wide; N may be any multiple of 16 (32 for a pair), so a block has as many columns as
+// the group has rows and no group pays for a row block it does not fill.  A group with more rows than a block takes is cut into
+// equal pieces (the plan kernel's list).  For few rows a stage is nearly all weight: the kernel then streams weights at the rate the
+// TMA unit fetches them, which is what bounds it.
+//   RB = 1: 128 weight columns a CTA, accumulators double-buffered in TMEM.  RB = 2: 2 x 128, which share the rows' tile (bytes fetched
+//   per flop are what bounds blocks of many rows); both halves of TMEM are then one block's.
+//   CTAS = 2: a cluster of two CTAs drives M = 256 MMAs, each CTA staging its own weight columns and half of the rows.
+//   NMAX: most rows of a block.  Few rows leave the shared memory to a deeper ring.
+// Roles, ring, bounded waits and hash tables of the producer are those of rz_tc_kernel.cuh.  Accumulator rows are weight columns, so
+// an epilogue thread owns one output column of 32 rows: bias is one value a thread, and 32 rows x 32 columns are transposed by
+// 2-byte stores into a tile of 64-byte rows (a warp's lanes are neighbours in the row: no bank conflicts), which a bulk tensor
+// store writes out; rows of a ragged end are stored one by one, since the rows behind belong to the next group.
+#pragma once
+#include "rz_common.h"
+#include "rz_ptx.cuh"
+
+using namespace rzptx;
+
+namespace {
+
+constexpr int ROWS_FWD = 0, ROWS_DX = 1;
+constexpr int ROWS_A_BLOCK = 16384;      // 128 weight columns x 64 contraction elements
+constexpr int ROWS_BATCH = 8;            // pipeline stages per hash batch of the producer warp
+constexpr int ROWS_MAX_BOXES = 8;        // weight boxes per stage at most
+constexpr int ROWS_MAX_STAGES = 10;
+constexpr int ROWS_SMEM_TABLE = 3 * ROWS_BATCH * ROWS_MAX_BOXES * 4;
+constexpr int ROWS_SMEM_BARS = (2 * ROWS_MAX_STAGES + 5) * 8;
+constexpr int ROWS_SMEM_LIMIT = 232448;
+constexpr int ROWS_TILE_BYTES = 2048;    // a warp's store tile: 32 rows x 32 columns
+
+__host__ __device__ constexpr int rows_stage_bytes(int ctas, int rb, int nmax) { return rb * ROWS_A_BLOCK + nmax / ctas * 128; }
+__host__ __device__ constexpr int rows_smem_fixed(int rb) { return 4 * rb * 2 * ROWS_TILE_BYTES + ROWS_SMEM_TABLE + ROWS_SMEM_BARS + 16 + 1024; }
+__host__ __device__ constexpr int rows_stages(int ctas, int rb, int nmax)
+{
+    const int n = (ROWS_SMEM_LIMIT - rows_smem_fixed(rb)) / rows_stage_bytes(ctas, rb, nmax);
+    return n > ROWS_MAX_STAGES ? ROWS_MAX_STAGES : n;
+}
+__host__ __device__ constexpr int rows_smem_total(int ctas, int rb, int nmax)
+{
+    return rows_stages(ctas, rb, nmax) * rows_stage_bytes(ctas, rb, nmax) + rows_smem_fixed(rb);
+}
+
+struct TcRowsParams {
+    RzHash hash;
+    const uint32_t *header;     // [0] = pieces
+    const uint4 *entries;       // {group, first row, end, 0} of each piece, at most NMAX rows
+    uint32_t group_tiles;       // hash-tile rows of one group's weight
+    uint32_t cols, tiles_c;     // output columns (the weight's N or K), blocks of them
+    uint32_t nchunks;           // pipeline stages of the contraction
+    uint32_t br, kparts;        // weight rows per box; FWD: boxes along a stage's contraction rows
+    uint32_t group_pieces;      // pieces per rasterisation group
+    float alpha;
+    int relu;
+    const float *bias;          // [groups][cols] or NULL
+    __nv_bfloat16 *out;
+    WaitCtx wait;
+};
+
+__device__ __forceinline__ void rows_wait_cycles(uint32_t bar, uint32_t parity, long long cycles)
+{
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity))
+        if (clock64() - t0 > cycles) break;
+}
+
+// mapW: shifted copies {element, slice row, copy}; mapR / mapRAll: the rows' matrix in boxes of 16 rows / of all rows a CTA stages
+// of a full block; mapC: the output in boxes of 32 x 32
+template <int OP, int CTAS, int RB, int NMAX>
+__global__ void __launch_bounds__(64 + 128 * RB, 1)
+rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapR,
+                  const __grid_constant__ CUtensorMap mapRAll, const __grid_constant__ CUtensorMap mapC, const TcRowsParams p)
+{
+    constexpr int KC = 64;                                    // contraction elements per stage: one 128-byte row
+    constexpr int STAGES = rows_stages(CTAS, RB, NMAX);
+    constexpr int STAGE_BYTES = rows_stage_bytes(CTAS, RB, NMAX);
+    constexpr int A_BYTES = RB * ROWS_A_BLOCK;
+    constexpr int PAIR_M = 128 * CTAS, ITEM_M = PAIR_M * RB;  // weight columns of an accumulator / of a block
+    constexpr int NBUF = 2 * RB * NMAX <= 512 ? 2 : 1;
+    constexpr int EPI_WARPS = 4 * RB;
+    constexpr uint32_t N_STEP = 16 * CTAS;                    // MMA N granularity
+    static_assert(STAGES >= 3, "ring");
+    static_assert(RB * NMAX <= 512 && NMAX % 32 == 0, "TMEM columns");
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    constexpr int RING = STAGES * STAGE_BYTES, TILES = EPI_WARPS * 2 * ROWS_TILE_BYTES;
+    uint32_t *tab_x = reinterpret_cast<uint32_t *>(smem_gen + RING + TILES);
+    uint32_t *tab_y = tab_x + ROWS_BATCH * ROWS_MAX_BOXES;
+    uint32_t *tab_z = tab_y + ROWS_BATCH * ROWS_MAX_BOXES;
+    const uint32_t bars = smem_base + RING + TILES + ROWS_SMEM_TABLE;
+    const uint32_t bar_full = bars;                                // [STAGES] used in the leader CTA
+    const uint32_t bar_empty = bars + 8 * ROWS_MAX_STAGES;         // [STAGES] one set per CTA
+    const uint32_t bar_tfull = bars + 16 * ROWS_MAX_STAGES;        // [2]      one set per CTA
+    const uint32_t bar_tempty = bars + 16 * ROWS_MAX_STAGES + 16;  // [2]      used in the leader CTA
+    const uint32_t bar_drain = bars + 16 * ROWS_MAX_STAGES + 32;   // [1]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem_gen + RING + TILES + ROWS_SMEM_TABLE + ROWS_SMEM_BARS);
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = (CTAS == 2) ? cluster_ctarank() : 0u;   // 0 = leader
+    const uint32_t first_item = (CTAS == 2) ? cluster_id_x() : blockIdx.x;
+    const uint32_t item_stride = gridDim.x / CTAS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(bar_tfull + 8 * b, 1);
+            mbar_init(bar_tempty + 8 * b, EPI_WARPS * CTAS);
+        }
+        mbar_init(bar_drain, 1);
+        fence_barrier_init();
+        fence_proxy_async();
+        tma_prefetch_desc(&mapW);
+        tma_prefetch_desc(&mapR);
+        tma_prefetch_desc(&mapRAll);
+        tma_prefetch_desc(&mapC);
+    }
+    if (warp == 1) {
+        if (CTAS == 2) {
+            tmem_alloc_pair(smem_u32(tmem_slot), 512);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_u32(tmem_slot), 512);
+            tmem_relinquish();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (CTAS == 2) cluster_sync_all();   // the peer's barriers exist before anything signals them
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
+
+    bool ok = true;
+    const uint32_t pieces = __ldg(p.header);
+    const uint32_t items = pieces * p.tiles_c;
+    uint32_t group = 0, row = 0, row_end = 0, width = 0, tc = 0;   // the block decoded last; width = its rows, as the MMA's N
+    // blocks are taken in groups of p.group_pieces pieces, column block after column block: the pieces of one group, which read the
+    // same weights, run side by side
+    auto decode = [&](uint32_t item) {
+        const uint32_t per_group = p.group_pieces * p.tiles_c;
+        const uint32_t g = item / per_group, within = item - g * per_group;
+        const uint32_t first = g * p.group_pieces, n = min(pieces - first, p.group_pieces);
+        tc = within / n;
+        const uint4 e = __ldg(p.entries + first + (within - tc * n));
+        group = e.x, row = e.y, row_end = e.z;
+        width = (row_end - row + N_STEP - 1) / N_STEP * N_STEP;
+    };
+
+    if (warp == 0) {
+        // ===================== producer (both CTAs of a pair) =====================
+        uint32_t it = 0;
+        uint32_t full_base = bar_full;
+        if (CTAS == 2) full_base = mapa_cluster(bar_full, 0);
+        const uint32_t boxes = (OP == ROWS_FWD) ? RB * 2 * p.kparts : RB * 128 / p.br;   // weight boxes per stage
+        const uint32_t box_bytes = p.br * 128u;
+        for (uint32_t item = first_item; item < items && ok; item += item_stride) {
+            decode(item);
+            const uint32_t staged = width / CTAS, row0 = row + rank * staged;   // rows this CTA stages
+            const uint32_t stage_tx = (uint32_t)CTAS * (A_BYTES + staged * 128u);
+            const uint32_t tile0 = group * p.group_tiles;
+            const uint32_t col0 = tc * ITEM_M + rank * 128;                     // weight columns of block r: col0 + r * PAIR_M
+            for (uint32_t cb = 0; cb < p.nchunks && ok; cb += ROWS_BATCH) {
+                const uint32_t nb = min((uint32_t)ROWS_BATCH, p.nchunks - cb);
+                for (uint32_t e = lane; e < nb * boxes; e += 32) {
+                    const uint32_t ci = e / boxes, j = e - ci * boxes;
+                    uint32_t pk, pn, x_in, y_in;
+                    if (OP == ROWS_FWD) {
+                        // box j = (row block r, 64 columns, part hh of the stage's contraction rows)
+                        const uint32_t ja = j / p.kparts, hh = j - ja * p.kparts;
+                        const uint32_t k0 = (cb + ci) * KC + hh * p.br, n = col0 + (ja >> 1) * PAIR_M + (ja & 1) * 64;
+                        pk = k0 / (uint32_t)p.hash.BK;
+                        y_in = k0 - pk * (uint32_t)p.hash.BK;
+                        pn = n / (uint32_t)p.hash.BN;
+                        x_in = n - pn * (uint32_t)p.hash.BN;
+                    } else {
+                        const uint32_t per_block = 128 / p.br, r = j / per_block;
+                        const uint32_t n0 = (cb + ci) * KC, ko = col0 + r * PAIR_M + (j - r * per_block) * p.br;
+                        pn = n0 / (uint32_t)p.hash.BN;
+                        x_in = n0 - pn * (uint32_t)p.hash.BN;
+                        pk = ko / (uint32_t)p.hash.BK;
+                        y_in = ko - pk * (uint32_t)p.hash.BK;
+                    }
+                    const uint32_t off = (uint32_t)rz_tile_offset(p.hash, tile0 + pk, pn), sh = off & 7u;
+                    tab_x[ci * ROWS_MAX_BOXES + j] = off - sh + x_in;
+                    tab_y[ci * ROWS_MAX_BOXES + j] = y_in;
+                    tab_z[ci * ROWS_MAX_BOXES + j] = sh;
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    for (uint32_t ci = 0; ci < nb; ++ci) {
+                        const uint32_t g = it + ci, s = g % STAGES, ph = (g / STAGES) & 1;
+                        if (!mbar_wait_bounded(bar_empty + 8 * s, ph ^ 1, RZ_WAIT_SMEM_EMPTY, p.wait, 2000)) {
+                            ok = false;
+                            it += ci;
+                            break;
+                        }
+                        const uint32_t full = full_base + 8 * s;
+                        const uint32_t sa = smem_base + s * STAGE_BYTES, sb = sa + A_BYTES;
+                        if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, stage_tx);
+                        for (uint32_t j = 0; j < boxes; ++j) {
+                            const int32_t x = (int32_t)tab_x[ci * ROWS_MAX_BOXES + j], y = (int32_t)tab_y[ci * ROWS_MAX_BOXES + j],
+                                          z = (int32_t)tab_z[ci * ROWS_MAX_BOXES + j];
+                            if (CTAS == 2) tma_load_3d_pair(sa + j * box_bytes, &mapW, full, x, y, z);
+                            else tma_load_3d(sa + j * box_bytes, &mapW, full, x, y, z);
+                        }
+                        const int32_t d0 = (int32_t)((cb + ci) * KC);
+                        if (staged == NMAX / CTAS) {
+                            if (CTAS == 2) tma_load_2d_pair(sb, &mapRAll, full, d0, (int32_t)row0);
+                            else tma_load_2d(sb, &mapRAll, full, d0, (int32_t)row0);
+                        } else {
+                            for (uint32_t r = 0; r < staged; r += 16) {
+                                if (CTAS == 2) tma_load_2d_pair(sb + r * 128, &mapR, full, d0, (int32_t)(row0 + r));
+                                else tma_load_2d(sb + r * 128, &mapR, full, d0, (int32_t)(row0 + r));
+                            }
+                        }
+                    }
+                    if (ok) it += nb;
+                }
+                __syncwarp();
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                it = __shfl_sync(0xffffffffu, it, 0);
+            }
+        }
+        if (!ok && lane == 0 && rank == 0) {
+            // give the loads already issued time to land before the CTA retires
+            const uint32_t lo = it > STAGES ? it - STAGES : 0;
+            for (uint32_t g = lo; g < it; ++g) rows_wait_cycles(bar_full + 8 * (g % STAGES), (g / STAGES) & 1, 4000000);
+        }
+    } else if (warp == 1) {
+        // ===================== MMA issuer (leader CTA only) =====================
+        constexpr uint32_t ATOM = KC * 128;   // bytes of a 64-column block of an M-major tile
+        constexpr uint32_t a_lbo = OP == ROWS_FWD ? ATOM : 16, a_kstep = OP == ROWS_FWD ? 16 * 128 : 32;
+        uint32_t it = 0, n_items = 0;
+        for (uint32_t item = first_item; item < items && ok && rank == 0; item += item_stride, ++n_items) {
+            decode(item);
+            const uint32_t buf = n_items % NBUF, tph = (n_items / NBUF) & 1;
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((OP == ROWS_FWD ? 1u : 0u) << 15) | ((width >> 3) << 17) |
+                                   ((uint32_t)(PAIR_M >> 4) << 24);
+            if (lane == 0) {
+                if (!mbar_wait_bounded(bar_tempty + 8 * buf, tph ^ 1, RZ_WAIT_TMEM_EMPTY, p.wait, 2000)) ok = false;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + buf * RB * NMAX;
+                for (uint32_t c = 0; c < p.nchunks && ok; ++c, ++it) {
+                    const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
+                    if (!mbar_wait_bounded(bar_full + 8 * s, ph, RZ_WAIT_SMEM_FULL, p.wait)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_base + s * STAGE_BYTES, sb = sa + A_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint64_t bd = make_desc_sw128(sb + kk * 32, 16, 1024, 2);
+                        const uint32_t acc = (c > 0 || kk > 0) ? 1u : 0u;
+#pragma unroll
+                        for (int r = 0; r < RB; ++r) {
+                            const uint64_t ad = make_desc_sw128(sa + r * ROWS_A_BLOCK + kk * a_kstep, a_lbo, 1024, 2);
+                            if (CTAS == 2) tc_mma_pair<false>(d_tmem + r * NMAX, ad, bd, idesc, acc);
+                            else tc_mma<false>(d_tmem + r * NMAX, ad, bd, idesc, acc);
+                        }
+                    }
+                    // frees this stage in both CTAs once the MMAs have read it
+                    if (CTAS == 2) tc_commit_pair(bar_empty + 8 * s, 3);
+                    else tc_commit(bar_empty + 8 * s);
+                }
+                if (ok) {
+                    if (CTAS == 2) tc_commit_pair(bar_tfull + 8 * buf, 3);
+                    else tc_commit(bar_tfull + 8 * buf);
+                }
+            }
+            __syncwarp();
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            it = __shfl_sync(0xffffffffu, it, 0);
+        }
+        if (!ok && lane == 0 && rank == 0) {
+            // MMAs may still be running: wait (bounded) until the tensor core has drained
+            if (CTAS == 2) tc_commit_pair(bar_drain, 1);
+            else tc_commit(bar_drain);
+            rows_wait_cycles(bar_drain, 0, 20000000);
+        }
+    } else {
+        // ===================== epilogue (both CTAs; each drains its own 128 weight columns) =====================
+        const uint32_t q = warp & 3;                 // TMEM lane quarter this warp may read
+        const uint32_t rblk = (warp - 2) >> 2;       // which accumulator of the block
+        uint8_t *tiles = smem_gen + RING + (warp - 2) * 2 * ROWS_TILE_BYTES;
+        uint32_t tempty_base = bar_tempty, flip = 0;
+        if (CTAS == 2) tempty_base = mapa_cluster(bar_tempty, 0);
+        uint32_t n_items = 0;
+        for (uint32_t item = first_item; item < items && ok; item += item_stride, ++n_items) {
+            decode(item);
+            const uint32_t buf = n_items % NBUF, tph = (n_items / NBUF) & 1;
+            const uint32_t cbase = tc * ITEM_M + rblk * PAIR_M + rank * 128 + q * 32, col = cbase + lane;   // this thread's output column
+            const bool col_ok = col < p.cols;
+            const float bias = p.bias && col_ok ? __ldg(p.bias + (size_t)group * p.cols + col) : 0.f;
+            bool mine = true;
+            if (lane == 0) mine = mbar_wait_bounded(bar_tfull + 8 * buf, tph, RZ_WAIT_TMEM_FULL, p.wait, 20000);
+            ok = __shfl_sync(0xffffffffu, (int)mine, 0) != 0;
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t acc = tmem_base + ((q * 32u) << 16) + (buf * RB + rblk) * NMAX;
+            const uint32_t chunks = (row_end - row + 31) / 32;
+            uint32_t next[32];
+            tmem_ld_32x32(acc, next);
+#pragma unroll 1
+            for (uint32_t c = 0; c < chunks; ++c) {
+                uint32_t v[32];
+                tmem_ld_wait_regs(next);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = next[j];
+                if (c + 1 < chunks) tmem_ld_32x32(acc + (c + 1) * 32, next);   // streams while this chunk is converted and stored
+                const uint32_t r0 = row + c * 32, rows = min(32u, row_end - r0);
+                uint16_t h[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    float f = __uint_as_float(v[j]) * p.alpha + bias;
+                    if (p.relu) f = fmaxf(f, 0.f);
+                    h[j] = __bfloat16_as_ushort(__float2bfloat16_rn(f));
+                }
+                if (rows == 32) {
+                    // the tile about to be rewritten: the store before the last must have read it
+                    if (lane == 0) bulk_wait_group_read1();
+                    __syncwarp();
+                    uint16_t *tile = reinterpret_cast<uint16_t *>(tiles + flip * ROWS_TILE_BYTES);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) tile[j * 32 + lane] = h[j];
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0 && cbase < p.cols) {
+                        tma_store_2d(&mapC, smem_u32(tile), (int32_t)cbase, (int32_t)r0);   // (columns past the matrix are clipped)
+                        bulk_commit_group();
+                    }
+                    flip ^= 1;
+                } else if (col_ok) {
+                    __nv_bfloat16 *o = p.out + (size_t)r0 * p.cols + col;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if ((uint32_t)j < rows) o[(size_t)j * p.cols] = __ushort_as_bfloat16(h[j]);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (CTAS == 2) mbar_arrive_cluster(tempty_base + 8 * buf);
+                else mbar_arrive(bar_tempty + 8 * buf);
+            }
+        }
+        if (lane == 0) bulk_wait_group0();   // bulk stores still in flight read this CTA's shared memory
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (CTAS == 2) cluster_sync_all();   // neither CTA retires while the peer may still signal or read it
+    if (warp == 1) {
+        tc_fence_after();
+        __syncwarp();
+        if (CTAS == 2) tmem_dealloc_pair(tmem_base, 512);
+        else tmem_dealloc(tmem_base, 512);
+    }
+}
+
+}  // namespace
