@@ -42,6 +42,7 @@ struct RzGroupPieces {
     const uint32_t *header = nullptr;   // [0] = how many there are
     const uint4 *entries = nullptr;     // {group, first row, end, 0}
     uint32_t most = 0;                  // the host's bound on header[0]
+    uint32_t groups = 0;
     uint32_t group_tiles = 0;           // hash-tile rows of one group's weight
 };
 

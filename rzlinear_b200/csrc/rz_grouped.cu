@@ -208,6 +208,7 @@ struct Plan {
         used += pieces_bytes(c.pb, groups, step);
         pieces.header = l.header, pieces.entries = l.entries;
         pieces.most = most_pieces(c.pb, groups, step);
+        pieces.groups = (uint32_t)groups;
         pieces.group_tiles = (uint32_t)((c.pb->K + c.pb->BK - 1) / c.pb->BK);
         return pieces;
     }

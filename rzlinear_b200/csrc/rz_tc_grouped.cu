@@ -81,10 +81,17 @@ int launch_persistent(Kernel kernel, int threads, int smem, int slots, uint64_t 
 // ---- bf16 products (rz_tc_rows.cuh) -----------------------------------------------------------------------------------------
 
 // weight rows per box: whole boxes per hash tile
-uint32_t rows_box(const rz_problem *pb, int op)
+uint32_t rows_box_log2(const rz_problem *pb, int op)
 {
-    if (pb->BK < 64) return 32;   // (BK is 32, 64 or a multiple of 64)
-    return op == RZ_OP_BACKWARD_INPUT && pb->BK % 128 == 0 ? 128 : 64;
+    if (pb->BK < 64) return 5;   // (BK is 32, 64 or a multiple of 64)
+    return op == RZ_OP_BACKWARD_INPUT && pb->BK % 128 == 0 ? 7 : 6;
+}
+
+int log2_or_none(int32_t v)
+{
+    int l = 0;
+    while (v >> l > 1) ++l;
+    return (1 << l) == v ? l : -1;
 }
 
 template <int OP, int CTAS, int RB, int NMAX>
@@ -100,8 +107,10 @@ int launch_rows(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *r
     p.cols = (uint32_t)cols;
     p.tiles_c = (uint32_t)((cols + 128 * CTAS * RB - 1) / (128 * CTAS * RB));
     p.nchunks = (uint32_t)((depth + 63) / 64);
-    p.br = rows_box(pb, op);
-    p.kparts = 64 / (p.br < 64 ? p.br : 64);
+    // (blocks and stages at the edges hash tiles a little beyond the last group's weight)
+    p.hash32 = rz_hash32(c.hash, (uint64_t)pieces.groups * pieces.group_tiles + 512 / 32, (uint64_t)(pb->N + pb->BN - 1) / pb->BN + 512 / 64);
+    p.bk_shift = log2_or_none(pb->BK), p.bn_shift = log2_or_none(pb->BN);
+    p.br_log2 = rows_box_log2(pb, op);
     p.group_pieces = 8;
     p.alpha = pb->alpha;
     p.relu = OP == ROWS_FWD && (pb->flags & RZ_FLAG_RELU) ? 1 : 0;
@@ -110,7 +119,7 @@ int launch_rows(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *r
     int st = rz_wait_context(&p.wait, 2000000000ll);   // also refuses to launch behind a kernel whose wait gave up
     if (st) return st;
     CUtensorMap mapW, mapR, mapRAll, mapC;
-    st = map_shadow(&mapW, pb, OP == ROWS_FWD, copies, p.br);
+    st = map_shadow(&mapW, pb, OP == ROWS_FWD, copies, 1u << p.br_log2);
     if (st) return st;
     st = map_matrix(&mapR, false, 0, rows, pb->M, depth, 64, 16);
     if (st) return st;
@@ -118,7 +127,7 @@ int launch_rows(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *r
     if (st) return st;
     st = map_matrix(&mapC, false, PLAIN_LAYOUT, out, pb->M, cols, 32, 32);
     if (st) return st;
-    constexpr int SMEM = rows_smem_total(CTAS, RB, NMAX), THREADS = 64 + 128 * RB;
+    constexpr int SMEM = rows_smem_total(CTAS, RB, NMAX), THREADS = rows_threads(RB);
     static_assert(SMEM <= ROWS_SMEM_LIMIT, "shared memory budget");
     int slots = 0;
     st = resident<rz_tc_rows_kernel<OP, CTAS, RB, NMAX>, CTAS>(pb, THREADS, SMEM, &slots);

@@ -9,7 +9,7 @@
 //   per flop are what bounds blocks of many rows); both halves of TMEM are then one block's.
 //   CTAS = 2: a cluster of two CTAs drives M = 256 MMAs, each CTA staging its own weight columns and half of the rows.
 //   NMAX: most rows of a block.  Few rows leave the shared memory to a deeper ring.
-// Roles, ring, bounded waits and hash tables of the producer are those of rz_tc_kernel.cuh.  Accumulator rows are weight columns, so
+// Roles, ring, bounded waits and hash tables of the producers are those of rz_tc_kernel.cuh, except that four warps produce.  Accumulator rows are weight columns, so
 // an epilogue thread owns one output column of 32 rows: bias is one value a thread, and 32 rows x 32 columns are transposed by
 // 2-byte stores into a tile of 64-byte rows (a warp's lanes are neighbours in the row: no bank conflicts), which a bulk tensor
 // store writes out; rows of a ragged end are stored one by one, since the rows behind belong to the next group.
@@ -23,10 +23,11 @@ namespace {
 
 constexpr int ROWS_FWD = 0, ROWS_DX = 1;
 constexpr int ROWS_A_BLOCK = 16384;      // 128 weight columns x 64 contraction elements
-constexpr int ROWS_BATCH = 8;            // pipeline stages per hash batch of the producer warp
+constexpr int ROWS_BATCH = 8;            // pipeline stages per hash batch of a producer warp
+constexpr int ROWS_PRODUCERS = 4;        // warps that issue loads
 constexpr int ROWS_MAX_BOXES = 8;        // weight boxes per stage at most
 constexpr int ROWS_MAX_STAGES = 10;
-constexpr int ROWS_SMEM_TABLE = 3 * ROWS_BATCH * ROWS_MAX_BOXES * 4;
+constexpr int ROWS_SMEM_TABLE = ROWS_BATCH * ROWS_MAX_BOXES * 8;
 constexpr int ROWS_SMEM_BARS = (2 * ROWS_MAX_STAGES + 5) * 8;
 constexpr int ROWS_SMEM_LIMIT = 232448;
 constexpr int ROWS_TILE_BYTES = 2048;    // a warp's store tile: 32 rows x 32 columns
@@ -43,14 +44,18 @@ __host__ __device__ constexpr int rows_smem_total(int ctas, int rb, int nmax)
     return rows_stages(ctas, rb, nmax) * rows_stage_bytes(ctas, rb, nmax) + rows_smem_fixed(rb);
 }
 
+__host__ __device__ constexpr int rows_threads(int rb) { return 32 * (1 + 4 * rb + ROWS_PRODUCERS); }
+
 struct TcRowsParams {
     RzHash hash;
+    RzHash32 hash32;
+    int bk_shift, bn_shift;     // log2 of the hash tile's sides, -1 for other sides
     const uint32_t *header;     // [0] = pieces
     const uint4 *entries;       // {group, first row, end, 0} of each piece, at most NMAX rows
     uint32_t group_tiles;       // hash-tile rows of one group's weight
     uint32_t cols, tiles_c;     // output columns (the weight's N or K), blocks of them
     uint32_t nchunks;           // pipeline stages of the contraction
-    uint32_t br, kparts;        // weight rows per box; FWD: boxes along a stage's contraction rows
+    uint32_t br_log2;           // weight rows per box: 32, 64 or 128
     uint32_t group_pieces;      // pieces per rasterisation group
     float alpha;
     int relu;
@@ -69,7 +74,7 @@ __device__ __forceinline__ void rows_wait_cycles(uint32_t bar, uint32_t parity, 
 // mapW: shifted copies {element, slice row, copy}; mapR / mapRAll: the rows' matrix in boxes of 16 rows / of all rows a CTA stages
 // of a full block; mapC: the output in boxes of 32 x 32
 template <int OP, int CTAS, int RB, int NMAX>
-__global__ void __launch_bounds__(64 + 128 * RB, 1)
+__global__ void __launch_bounds__(rows_threads(RB), 1)
 rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapR,
                   const __grid_constant__ CUtensorMap mapRAll, const __grid_constant__ CUtensorMap mapC, const TcRowsParams p)
 {
@@ -88,9 +93,7 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     constexpr int RING = STAGES * STAGE_BYTES, TILES = EPI_WARPS * 2 * ROWS_TILE_BYTES;
-    uint32_t *tab_x = reinterpret_cast<uint32_t *>(smem_gen + RING + TILES);
-    uint32_t *tab_y = tab_x + ROWS_BATCH * ROWS_MAX_BOXES;
-    uint32_t *tab_z = tab_y + ROWS_BATCH * ROWS_MAX_BOXES;
+    uint2 *table = reinterpret_cast<uint2 *>(smem_gen + RING + TILES);   // a box: element in a copy, slice row << 3 | copy
     const uint32_t bars = smem_base + RING + TILES + ROWS_SMEM_TABLE;
     const uint32_t bar_full = bars;                                // [STAGES] used in the leader CTA
     const uint32_t bar_empty = bars + 8 * ROWS_MAX_STAGES;         // [STAGES] one set per CTA
@@ -152,82 +155,94 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
         width = (row_end - row + N_STEP - 1) / N_STEP * N_STEP;
     };
 
-    if (warp == 0) {
-        // ===================== producer (both CTAs of a pair) =====================
-        uint32_t it = 0;
+    if (warp == 0 || warp >= 2 + EPI_WARPS) {
+        // ===================== producers (both CTAs of a pair) =====================
+        // One thread takes some 130 clocks to issue a load, and a stage has up to 8 weight boxes and 16 boxes of rows: four warps
+        // share them, box by box.
+        const uint32_t which = warp == 0 ? 0u : warp - (1 + EPI_WARPS);   // 0 .. ROWS_PRODUCERS - 1
+        uint2 *mine_table = table + which * (ROWS_BATCH * ROWS_MAX_BOXES / ROWS_PRODUCERS);
+        uint32_t it = 0, slot = 0, phase = 1;   // stages issued; the ring's next slot, and the parity that says it is free
         uint32_t full_base = bar_full;
         if (CTAS == 2) full_base = mapa_cluster(bar_full, 0);
-        const uint32_t boxes = (OP == ROWS_FWD) ? RB * 2 * p.kparts : RB * 128 / p.br;   // weight boxes per stage
-        const uint32_t box_bytes = p.br * 128u;
+        // The hash table of a batch is what this warp spends most of its time on when stages are short, so it is computed in 32 bits
+        // where possible and without divisions.
+        auto tile_of = [](uint32_t v, uint32_t side, int shift) { return shift >= 0 ? v >> shift : v / side; };
+        constexpr uint32_t RB_LOG2 = RB - 1;   // (RB is 1 or 2)
+        const uint32_t br = 1u << p.br_log2, per_block_log2 = 7 - p.br_log2;
+        const uint32_t boxes_log2 = RB_LOG2 + per_block_log2, boxes = 1u << boxes_log2, box_bytes = br * 128u;
+        const uint32_t mine_boxes = boxes > which ? (boxes - which + ROWS_PRODUCERS - 1) / ROWS_PRODUCERS : 0u;   // which, which + 4: at most two
+        const uint32_t mine_log2 = mine_boxes > 1 ? 1u : 0u;
+        const uint32_t dst0 = which * box_bytes, dst1 = (which + ROWS_PRODUCERS) * box_bytes;
+        const uint32_t first_r = (ROWS_PRODUCERS - 1 - which) * 16;   // rows' boxes: the last producer first, it has the fewest weight boxes
         for (uint32_t item = first_item; item < items && ok; item += item_stride) {
             decode(item);
             const uint32_t staged = width / CTAS, row0 = row + rank * staged;   // rows this CTA stages
             const uint32_t stage_tx = (uint32_t)CTAS * (A_BYTES + staged * 128u);
+            const bool whole = staged == NMAX / CTAS;   // all rows of a stage come in one box
             const uint32_t tile0 = group * p.group_tiles;
             const uint32_t col0 = tc * ITEM_M + rank * 128;                     // weight columns of block r: col0 + r * PAIR_M
             for (uint32_t cb = 0; cb < p.nchunks && ok; cb += ROWS_BATCH) {
                 const uint32_t nb = min((uint32_t)ROWS_BATCH, p.nchunks - cb);
-                for (uint32_t e = lane; e < nb * boxes; e += 32) {
-                    const uint32_t ci = e / boxes, j = e - ci * boxes;
-                    uint32_t pk, pn, x_in, y_in;
+                if (mine_boxes && lane < nb << mine_log2) {
+                    const uint32_t ci = lane >> mine_log2, j = which + (lane & mine_log2) * ROWS_PRODUCERS;
+                    const uint32_t r = j >> per_block_log2, i = j & ((1u << per_block_log2) - 1);
+                    uint32_t k, n;   // first weight row and column of the box
                     if (OP == ROWS_FWD) {
-                        // box j = (row block r, 64 columns, part hh of the stage's contraction rows)
-                        const uint32_t ja = j / p.kparts, hh = j - ja * p.kparts;
-                        const uint32_t k0 = (cb + ci) * KC + hh * p.br, n = col0 + (ja >> 1) * PAIR_M + (ja & 1) * 64;
-                        pk = k0 / (uint32_t)p.hash.BK;
-                        y_in = k0 - pk * (uint32_t)p.hash.BK;
-                        pn = n / (uint32_t)p.hash.BN;
-                        x_in = n - pn * (uint32_t)p.hash.BN;
+                        // boxes of a block: two halves of 64 columns, each in 64 / br parts along the contraction (br <= 64)
+                        const uint32_t parts_log2 = 6 - p.br_log2;
+                        n = col0 + r * PAIR_M + (i >> parts_log2) * 64;
+                        k = (cb + ci) * KC + (i & ((1u << parts_log2) - 1)) * br;
                     } else {
-                        const uint32_t per_block = 128 / p.br, r = j / per_block;
-                        const uint32_t n0 = (cb + ci) * KC, ko = col0 + r * PAIR_M + (j - r * per_block) * p.br;
-                        pn = n0 / (uint32_t)p.hash.BN;
-                        x_in = n0 - pn * (uint32_t)p.hash.BN;
-                        pk = ko / (uint32_t)p.hash.BK;
-                        y_in = ko - pk * (uint32_t)p.hash.BK;
+                        n = (cb + ci) * KC;
+                        k = col0 + r * PAIR_M + i * br;
                     }
-                    const uint32_t off = (uint32_t)rz_tile_offset(p.hash, tile0 + pk, pn), sh = off & 7u;
-                    tab_x[ci * ROWS_MAX_BOXES + j] = off - sh + x_in;
-                    tab_y[ci * ROWS_MAX_BOXES + j] = y_in;
-                    tab_z[ci * ROWS_MAX_BOXES + j] = sh;
+                    const uint32_t pk = tile_of(k, (uint32_t)p.hash.BK, p.bk_shift), pn = tile_of(n, (uint32_t)p.hash.BN, p.bn_shift);
+                    const uint32_t off = rz_tile_offset32(p.hash, p.hash32, tile0 + pk, pn), sh = off & 7u;
+                    mine_table[lane] = make_uint2(off - sh + (n - pn * (uint32_t)p.hash.BN), (k - pk * (uint32_t)p.hash.BK) << 3 | sh);
                 }
                 __syncwarp();
+                // One thread, instruction after instruction at some five clocks each: everything that can be is kept in registers.
                 if (lane == 0) {
-                    for (uint32_t ci = 0; ci < nb; ++ci) {
-                        const uint32_t g = it + ci, s = g % STAGES, ph = (g / STAGES) & 1;
-                        if (!mbar_wait_bounded(bar_empty + 8 * s, ph ^ 1, RZ_WAIT_SMEM_EMPTY, p.wait, 2000)) {
+                    uint2 box0 = mine_table[0], box1 = mine_table[mine_log2];
+                    int32_t d0 = (int32_t)(cb * KC);
+                    for (uint32_t ci = 0; ci < nb; ++ci, d0 += KC) {
+                        if (!mbar_wait_bounded(bar_empty + 8 * slot, phase, RZ_WAIT_SMEM_EMPTY, p.wait, 2000)) {
                             ok = false;
-                            it += ci;
                             break;
                         }
-                        const uint32_t full = full_base + 8 * s;
-                        const uint32_t sa = smem_base + s * STAGE_BYTES, sb = sa + A_BYTES;
-                        if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, stage_tx);
-                        for (uint32_t j = 0; j < boxes; ++j) {
-                            const int32_t x = (int32_t)tab_x[ci * ROWS_MAX_BOXES + j], y = (int32_t)tab_y[ci * ROWS_MAX_BOXES + j],
-                                          z = (int32_t)tab_z[ci * ROWS_MAX_BOXES + j];
-                            if (CTAS == 2) tma_load_3d_pair(sa + j * box_bytes, &mapW, full, x, y, z);
-                            else tma_load_3d(sa + j * box_bytes, &mapW, full, x, y, z);
+                        const uint32_t full = full_base + 8 * slot, sa = smem_base + slot * STAGE_BYTES, sb = sa + A_BYTES;
+                        if (rank == 0 && which == 0) mbar_arrive_expect_tx(bar_full + 8 * slot, stage_tx);
+                        if (mine_boxes > 0) {
+                            if (CTAS == 2) tma_load_3d_pair(sa + dst0, &mapW, full, (int32_t)box0.x, (int32_t)(box0.y >> 3), (int32_t)(box0.y & 7u));
+                            else tma_load_3d(sa + dst0, &mapW, full, (int32_t)box0.x, (int32_t)(box0.y >> 3), (int32_t)(box0.y & 7u));
                         }
-                        const int32_t d0 = (int32_t)((cb + ci) * KC);
-                        if (staged == NMAX / CTAS) {
-                            if (CTAS == 2) tma_load_2d_pair(sb, &mapRAll, full, d0, (int32_t)row0);
-                            else tma_load_2d(sb, &mapRAll, full, d0, (int32_t)row0);
+                        if (mine_boxes > 1) {
+                            if (CTAS == 2) tma_load_3d_pair(sa + dst1, &mapW, full, (int32_t)box1.x, (int32_t)(box1.y >> 3), (int32_t)(box1.y & 7u));
+                            else tma_load_3d(sa + dst1, &mapW, full, (int32_t)box1.x, (int32_t)(box1.y >> 3), (int32_t)(box1.y & 7u));
+                        }
+                        if (whole) {
+                            if (which == ROWS_PRODUCERS - 1) {
+                                if (CTAS == 2) tma_load_2d_pair(sb, &mapRAll, full, d0, (int32_t)row0);
+                                else tma_load_2d(sb, &mapRAll, full, d0, (int32_t)row0);
+                            }
                         } else {
-                            for (uint32_t r = 0; r < staged; r += 16) {
+#pragma unroll 1
+                            for (uint32_t r = first_r; r < staged; r += ROWS_PRODUCERS * 16) {
                                 if (CTAS == 2) tma_load_2d_pair(sb + r * 128, &mapR, full, d0, (int32_t)(row0 + r));
                                 else tma_load_2d(sb + r * 128, &mapR, full, d0, (int32_t)(row0 + r));
                             }
                         }
+                        const uint32_t next = min(ci + 1, nb - 1) << mine_log2;
+                        box0 = mine_table[next], box1 = mine_table[next + mine_log2];
+                        ++it;
+                        if (++slot == STAGES) slot = 0, phase ^= 1u;
                     }
-                    if (ok) it += nb;
                 }
                 __syncwarp();
                 ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-                it = __shfl_sync(0xffffffffu, it, 0);
             }
         }
-        if (!ok && lane == 0 && rank == 0) {
+        if (!ok && lane == 0 && rank == 0) {   // (`it` counts in this thread)
             // give the loads already issued time to land before the CTA retires
             const uint32_t lo = it > STAGES ? it - STAGES : 0;
             for (uint32_t g = lo; g < it; ++g) rows_wait_cycles(bar_full + 8 * (g % STAGES), (g / STAGES) & 1, 4000000);
@@ -236,7 +251,10 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
         // ===================== MMA issuer (leader CTA only) =====================
         constexpr uint32_t ATOM = KC * 128;   // bytes of a 64-column block of an M-major tile
         constexpr uint32_t a_lbo = OP == ROWS_FWD ? ATOM : 16, a_kstep = OP == ROWS_FWD ? 16 * 128 : 32;
-        uint32_t it = 0, n_items = 0;
+        // descriptors differ in their low words only, by sixteenths of the address (which stays below 2^18)
+        const uint64_t a0 = make_desc_sw128(smem_base, a_lbo, 1024, 2), b0 = make_desc_sw128(smem_base + A_BYTES, 16, 1024, 2);
+        const uint32_t a_lo = (uint32_t)a0, a_hi = (uint32_t)(a0 >> 32), b_lo = (uint32_t)b0, b_hi = (uint32_t)(b0 >> 32);
+        uint32_t n_items = 0, slot = 0, phase = 0;
         for (uint32_t item = first_item; item < items && ok && rank == 0; item += item_stride, ++n_items) {
             decode(item);
             const uint32_t buf = n_items % NBUF, tph = (n_items / NBUF) & 1;
@@ -246,28 +264,30 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
                 if (!mbar_wait_bounded(bar_tempty + 8 * buf, tph ^ 1, RZ_WAIT_TMEM_EMPTY, p.wait, 2000)) ok = false;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + buf * RB * NMAX;
-                for (uint32_t c = 0; c < p.nchunks && ok; ++c, ++it) {
-                    const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
-                    if (!mbar_wait_bounded(bar_full + 8 * s, ph, RZ_WAIT_SMEM_FULL, p.wait)) {
+                uint32_t acc = 0;
+#pragma unroll 1
+                for (uint32_t c = 0; c < p.nchunks && ok; ++c) {
+                    if (!mbar_wait_bounded(bar_full + 8 * slot, phase, RZ_WAIT_SMEM_FULL, p.wait)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_base + s * STAGE_BYTES, sb = sa + A_BYTES;
+                    const uint32_t al = a_lo + slot * (STAGE_BYTES / 16), bl = b_lo + slot * (STAGE_BYTES / 16);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t bd = make_desc_sw128(sb + kk * 32, 16, 1024, 2);
-                        const uint32_t acc = (c > 0 || kk > 0) ? 1u : 0u;
+                        const uint64_t bd = (uint64_t)b_hi << 32 | (bl + kk * (32 / 16));
 #pragma unroll
                         for (int r = 0; r < RB; ++r) {
-                            const uint64_t ad = make_desc_sw128(sa + r * ROWS_A_BLOCK + kk * a_kstep, a_lbo, 1024, 2);
+                            const uint64_t ad = (uint64_t)a_hi << 32 | (al + (r * ROWS_A_BLOCK + kk * a_kstep) / 16);
                             if (CTAS == 2) tc_mma_pair<false>(d_tmem + r * NMAX, ad, bd, idesc, acc);
                             else tc_mma<false>(d_tmem + r * NMAX, ad, bd, idesc, acc);
                         }
+                        acc = 1;
                     }
                     // frees this stage in both CTAs once the MMAs have read it
-                    if (CTAS == 2) tc_commit_pair(bar_empty + 8 * s, 3);
-                    else tc_commit(bar_empty + 8 * s);
+                    if (CTAS == 2) tc_commit_pair(bar_empty + 8 * slot, 3);
+                    else tc_commit(bar_empty + 8 * slot);
+                    if (++slot == STAGES) slot = 0, phase ^= 1u;
                 }
                 if (ok) {
                     if (CTAS == 2) tc_commit_pair(bar_tfull + 8 * buf, 3);
@@ -276,7 +296,6 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
             }
             __syncwarp();
             ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-            it = __shfl_sync(0xffffffffu, it, 0);
         }
         if (!ok && lane == 0 && rank == 0) {
             // MMAs may still be running: wait (bounded) until the tensor core has drained
