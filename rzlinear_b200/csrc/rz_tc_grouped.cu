@@ -118,10 +118,12 @@ int launch_rows(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *r
     p.out = static_cast<__nv_bfloat16 *>(out);
     int st = rz_wait_context(&p.wait, 2000000000ll);   // also refuses to launch behind a kernel whose wait gave up
     if (st) return st;
-    CUtensorMap mapW, mapR, mapRAll, mapC;
+    CUtensorMap mapW, mapR16, mapR64, mapRAll, mapC;
     st = map_shadow(&mapW, pb, OP == ROWS_FWD, copies, 1u << p.br_log2);
     if (st) return st;
-    st = map_matrix(&mapR, false, 0, rows, pb->M, depth, 64, 16);
+    st = map_matrix(&mapR16, false, 0, rows, pb->M, depth, 64, 16);
+    if (st) return st;
+    st = map_matrix(&mapR64, false, 0, rows, pb->M, depth, 64, 64);
     if (st) return st;
     st = map_matrix(&mapRAll, false, 0, rows, pb->M, depth, 64, NMAX / CTAS);
     if (st) return st;
@@ -133,7 +135,7 @@ int launch_rows(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *r
     st = resident<rz_tc_rows_kernel<OP, CTAS, RB, NMAX>, CTAS>(pb, THREADS, SMEM, &slots);
     if (st) return st;
     return launch_persistent<CTAS>(rz_tc_rows_kernel<OP, CTAS, RB, NMAX>, THREADS, SMEM, slots, (uint64_t)pieces.most * p.tiles_c, c.stream, mapW,
-                                   mapR, mapRAll, mapC, p);
+                                   mapR16, mapR64, mapRAll, mapC, p);
 }
 
 template <int OP>

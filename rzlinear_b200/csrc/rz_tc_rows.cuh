@@ -23,11 +23,11 @@ namespace {
 
 constexpr int ROWS_FWD = 0, ROWS_DX = 1;
 constexpr int ROWS_A_BLOCK = 16384;      // 128 weight columns x 64 contraction elements
-constexpr int ROWS_BATCH = 8;            // pipeline stages per hash batch of a producer warp
+constexpr int ROWS_BATCH = 4;            // pipeline stages per hash batch of a producer warp
 constexpr int ROWS_PRODUCERS = 4;        // warps that issue loads
 constexpr int ROWS_MAX_BOXES = 8;        // weight boxes per stage at most
 constexpr int ROWS_MAX_STAGES = 10;
-constexpr int ROWS_SMEM_TABLE = ROWS_BATCH * ROWS_MAX_BOXES * 8;
+constexpr int ROWS_SMEM_TABLE = ROWS_PRODUCERS * ROWS_BATCH * ROWS_MAX_BOXES * 8;
 constexpr int ROWS_SMEM_BARS = (2 * ROWS_MAX_STAGES + 5) * 8;
 constexpr int ROWS_SMEM_LIMIT = 232448;
 constexpr int ROWS_TILE_BYTES = 2048;    // a warp's store tile: 32 rows x 32 columns
@@ -71,12 +71,12 @@ __device__ __forceinline__ void rows_wait_cycles(uint32_t bar, uint32_t parity, 
         if (clock64() - t0 > cycles) break;
 }
 
-// mapW: shifted copies {element, slice row, copy}; mapR / mapRAll: the rows' matrix in boxes of 16 rows / of all rows a CTA stages
-// of a full block; mapC: the output in boxes of 32 x 32
+// mapW: shifted copies {element, slice row, copy}; mapR16, 64, All: the rows' matrix in boxes of 16 rows, 64 rows and all the rows
+// that a CTA stages of a full block; mapC: the output in boxes of 32 x 32
 template <int OP, int CTAS, int RB, int NMAX>
 __global__ void __launch_bounds__(rows_threads(RB), 1)
-rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapR,
-                  const __grid_constant__ CUtensorMap mapRAll, const __grid_constant__ CUtensorMap mapC, const TcRowsParams p)
+rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapR16,
+                  const __grid_constant__ CUtensorMap mapR64, const __grid_constant__ CUtensorMap mapRAll, const __grid_constant__ CUtensorMap mapC, const TcRowsParams p)
 {
     constexpr int KC = 64;                                    // contraction elements per stage: one 128-byte row
     constexpr int STAGES = rows_stages(CTAS, RB, NMAX);
@@ -93,7 +93,6 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     constexpr int RING = STAGES * STAGE_BYTES, TILES = EPI_WARPS * 2 * ROWS_TILE_BYTES;
-    uint2 *table = reinterpret_cast<uint2 *>(smem_gen + RING + TILES);   // a box: element in a copy, slice row << 3 | copy
     const uint32_t bars = smem_base + RING + TILES + ROWS_SMEM_TABLE;
     const uint32_t bar_full = bars;                                // [STAGES] used in the leader CTA
     const uint32_t bar_empty = bars + 8 * ROWS_MAX_STAGES;         // [STAGES] one set per CTA
@@ -120,7 +119,8 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
         fence_barrier_init();
         fence_proxy_async();
         tma_prefetch_desc(&mapW);
-        tma_prefetch_desc(&mapR);
+        tma_prefetch_desc(&mapR16);
+        tma_prefetch_desc(&mapR64);
         tma_prefetch_desc(&mapRAll);
         tma_prefetch_desc(&mapC);
     }
@@ -157,95 +157,93 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
 
     if (warp == 0 || warp >= 2 + EPI_WARPS) {
         // ===================== producers (both CTAs of a pair) =====================
-        // One thread takes some 130 clocks to issue a load, and a stage has up to 8 weight boxes and 16 boxes of rows: four warps
-        // share them, box by box.
+        // A stage costs its producer some 300 clocks and 130 for each of its boxes (one thread, instruction after instruction), more
+        // than the TMA unit or the tensor core needs for short stages: four warps take the stages in turn.
         const uint32_t which = warp == 0 ? 0u : warp - (1 + EPI_WARPS);   // 0 .. ROWS_PRODUCERS - 1
-        uint2 *mine_table = table + which * (ROWS_BATCH * ROWS_MAX_BOXES / ROWS_PRODUCERS);
-        uint32_t it = 0, slot = 0, phase = 1;   // stages issued; the ring's next slot, and the parity that says it is free
+        uint2 *mine = reinterpret_cast<uint2 *>(smem_gen + RING + TILES) + which * (ROWS_BATCH * ROWS_MAX_BOXES);   // boxes: element in a copy, slice row << 3 | copy
+        auto tile_of = [](uint32_t v, uint32_t side, int shift) { return shift >= 0 ? v >> shift : v / side; };
+        const uint32_t br = 1u << p.br_log2, per_block_log2 = 7 - p.br_log2;
+        const uint32_t boxes_log2 = (RB - 1) + per_block_log2, boxes = 1u << boxes_log2, box_bytes = br * 128u;   // (RB is 1 or 2)
         uint32_t full_base = bar_full;
         if (CTAS == 2) full_base = mapa_cluster(bar_full, 0);
-        // The hash table of a batch is what this warp spends most of its time on when stages are short, so it is computed in 32 bits
-        // where possible and without divisions.
-        auto tile_of = [](uint32_t v, uint32_t side, int shift) { return shift >= 0 ? v >> shift : v / side; };
-        constexpr uint32_t RB_LOG2 = RB - 1;   // (RB is 1 or 2)
-        const uint32_t br = 1u << p.br_log2, per_block_log2 = 7 - p.br_log2;
-        const uint32_t boxes_log2 = RB_LOG2 + per_block_log2, boxes = 1u << boxes_log2, box_bytes = br * 128u;
-        const uint32_t mine_boxes = boxes > which ? (boxes - which + ROWS_PRODUCERS - 1) / ROWS_PRODUCERS : 0u;   // which, which + 4: at most two
-        const uint32_t mine_log2 = mine_boxes > 1 ? 1u : 0u;
-        const uint32_t dst0 = which * box_bytes, dst1 = (which + ROWS_PRODUCERS) * box_bytes;
-        const uint32_t first_r = (ROWS_PRODUCERS - 1 - which) * 16;   // rows' boxes: the last producer first, it has the fewest weight boxes
+        uint32_t slot = which % STAGES, phase = (which / STAGES & 1) ^ 1;   // this warp's next slot of the ring, and the parity that says it is free
+        uint32_t skip = which;                                              // stages of other producers before this warp's next one
         for (uint32_t item = first_item; item < items && ok; item += item_stride) {
             decode(item);
             const uint32_t staged = width / CTAS, row0 = row + rank * staged;   // rows this CTA stages
             const uint32_t stage_tx = (uint32_t)CTAS * (A_BYTES + staged * 128u);
-            const bool whole = staged == NMAX / CTAS;   // all rows of a stage come in one box
             const uint32_t tile0 = group * p.group_tiles;
             const uint32_t col0 = tc * ITEM_M + rank * 128;                     // weight columns of block r: col0 + r * PAIR_M
-            for (uint32_t cb = 0; cb < p.nchunks && ok; cb += ROWS_BATCH) {
-                const uint32_t nb = min((uint32_t)ROWS_BATCH, p.nchunks - cb);
-                if (mine_boxes && lane < nb << mine_log2) {
-                    const uint32_t ci = lane >> mine_log2, j = which + (lane & mine_log2) * ROWS_PRODUCERS;
+            uint32_t c = skip;
+            while (c < p.nchunks && ok) {
+                const uint32_t nb = min((uint32_t)ROWS_BATCH, (p.nchunks - c + ROWS_PRODUCERS - 1) / ROWS_PRODUCERS);
+                __syncwarp();
+                // the boxes' places, a batch of this warp's stages at once; in 32 bits where possible, and without divisions
+                for (uint32_t e = lane; e < nb << boxes_log2; e += 32) {
+                    const uint32_t stage = c + (e >> boxes_log2) * ROWS_PRODUCERS, j = e & (boxes - 1);
                     const uint32_t r = j >> per_block_log2, i = j & ((1u << per_block_log2) - 1);
                     uint32_t k, n;   // first weight row and column of the box
                     if (OP == ROWS_FWD) {
                         // boxes of a block: two halves of 64 columns, each in 64 / br parts along the contraction (br <= 64)
                         const uint32_t parts_log2 = 6 - p.br_log2;
                         n = col0 + r * PAIR_M + (i >> parts_log2) * 64;
-                        k = (cb + ci) * KC + (i & ((1u << parts_log2) - 1)) * br;
+                        k = stage * KC + (i & ((1u << parts_log2) - 1)) * br;
                     } else {
-                        n = (cb + ci) * KC;
+                        n = stage * KC;
                         k = col0 + r * PAIR_M + i * br;
                     }
                     const uint32_t pk = tile_of(k, (uint32_t)p.hash.BK, p.bk_shift), pn = tile_of(n, (uint32_t)p.hash.BN, p.bn_shift);
                     const uint32_t off = rz_tile_offset32(p.hash, p.hash32, tile0 + pk, pn), sh = off & 7u;
-                    mine_table[lane] = make_uint2(off - sh + (n - pn * (uint32_t)p.hash.BN), (k - pk * (uint32_t)p.hash.BK) << 3 | sh);
+                    mine[e] = make_uint2(off - sh + (n - pn * (uint32_t)p.hash.BN), (k - pk * (uint32_t)p.hash.BK) << 3 | sh);
                 }
                 __syncwarp();
-                // One thread, instruction after instruction at some five clocks each: everything that can be is kept in registers.
                 if (lane == 0) {
-                    uint2 box0 = mine_table[0], box1 = mine_table[mine_log2];
-                    int32_t d0 = (int32_t)(cb * KC);
-                    for (uint32_t ci = 0; ci < nb; ++ci, d0 += KC) {
+                    for (uint32_t ci = 0; ci < nb; ++ci) {
                         if (!mbar_wait_bounded(bar_empty + 8 * slot, phase, RZ_WAIT_SMEM_EMPTY, p.wait, 2000)) {
                             ok = false;
                             break;
                         }
-                        const uint32_t full = full_base + 8 * slot, sa = smem_base + slot * STAGE_BYTES, sb = sa + A_BYTES;
-                        if (rank == 0 && which == 0) mbar_arrive_expect_tx(bar_full + 8 * slot, stage_tx);
-                        if (mine_boxes > 0) {
-                            if (CTAS == 2) tma_load_3d_pair(sa + dst0, &mapW, full, (int32_t)box0.x, (int32_t)(box0.y >> 3), (int32_t)(box0.y & 7u));
-                            else tma_load_3d(sa + dst0, &mapW, full, (int32_t)box0.x, (int32_t)(box0.y >> 3), (int32_t)(box0.y & 7u));
-                        }
-                        if (mine_boxes > 1) {
-                            if (CTAS == 2) tma_load_3d_pair(sa + dst1, &mapW, full, (int32_t)box1.x, (int32_t)(box1.y >> 3), (int32_t)(box1.y & 7u));
-                            else tma_load_3d(sa + dst1, &mapW, full, (int32_t)box1.x, (int32_t)(box1.y >> 3), (int32_t)(box1.y & 7u));
-                        }
-                        if (whole) {
-                            if (which == ROWS_PRODUCERS - 1) {
-                                if (CTAS == 2) tma_load_2d_pair(sb, &mapRAll, full, d0, (int32_t)row0);
-                                else tma_load_2d(sb, &mapRAll, full, d0, (int32_t)row0);
-                            }
-                        } else {
+                        const uint32_t full = full_base + 8 * slot;
+                        uint32_t dst = smem_base + slot * STAGE_BYTES;
+                        if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * slot, stage_tx);
 #pragma unroll 1
-                            for (uint32_t r = first_r; r < staged; r += ROWS_PRODUCERS * 16) {
-                                if (CTAS == 2) tma_load_2d_pair(sb + r * 128, &mapR, full, d0, (int32_t)(row0 + r));
-                                else tma_load_2d(sb + r * 128, &mapR, full, d0, (int32_t)(row0 + r));
+                        for (uint32_t j = 0; j < boxes; ++j, dst += box_bytes) {
+                            const uint2 u = mine[(ci << boxes_log2) + j];
+                            if (CTAS == 2) tma_load_3d_pair(dst, &mapW, full, (int32_t)u.x, (int32_t)(u.y >> 3), (int32_t)(u.y & 7u));
+                            else tma_load_3d(dst, &mapW, full, (int32_t)u.x, (int32_t)(u.y >> 3), (int32_t)(u.y & 7u));
+                        }
+                        const int32_t d0 = (int32_t)((c + ci * ROWS_PRODUCERS) * KC);
+                        if (staged == NMAX / CTAS) {
+                            if (CTAS == 2) tma_load_2d_pair(dst, &mapRAll, full, d0, (int32_t)row0);
+                            else tma_load_2d(dst, &mapRAll, full, d0, (int32_t)row0);
+                        } else {
+                            uint32_t r = 0;
+#pragma unroll 1
+                            for (; r + 64 <= staged; r += 64) {
+                                if (CTAS == 2) tma_load_2d_pair(dst + r * 128, &mapR64, full, d0, (int32_t)(row0 + r));
+                                else tma_load_2d(dst + r * 128, &mapR64, full, d0, (int32_t)(row0 + r));
+                            }
+#pragma unroll 1
+                            for (; r < staged; r += 16) {
+                                if (CTAS == 2) tma_load_2d_pair(dst + r * 128, &mapR16, full, d0, (int32_t)(row0 + r));
+                                else tma_load_2d(dst + r * 128, &mapR16, full, d0, (int32_t)(row0 + r));
                             }
                         }
-                        const uint32_t next = min(ci + 1, nb - 1) << mine_log2;
-                        box0 = mine_table[next], box1 = mine_table[next + mine_log2];
-                        ++it;
-                        if (++slot == STAGES) slot = 0, phase ^= 1u;
+                        for (slot += ROWS_PRODUCERS; slot >= STAGES; slot -= STAGES) phase ^= 1u;
                     }
                 }
                 __syncwarp();
                 ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                c += nb * ROWS_PRODUCERS;
             }
+            skip = c - p.nchunks;
         }
-        if (!ok && lane == 0 && rank == 0) {   // (`it` counts in this thread)
-            // give the loads already issued time to land before the CTA retires
-            const uint32_t lo = it > STAGES ? it - STAGES : 0;
-            for (uint32_t g = lo; g < it; ++g) rows_wait_cycles(bar_full + 8 * (g % STAGES), (g / STAGES) & 1, 4000000);
+        if (!ok && lane == 0 && rank == 0) {
+            // give the loads already issued time to land before the CTA retires: a stage's barrier ends the phase it was armed in
+            for (uint32_t s = 0; s < STAGES; ++s) {
+                rows_wait_cycles(bar_full + 8 * s, 0, 2000000);
+                rows_wait_cycles(bar_full + 8 * s, 1, 2000000);
+            }
         }
     } else if (warp == 1) {
         // ===================== MMA issuer (leader CTA only) =====================
