@@ -142,20 +142,23 @@ template <int OP>
 int launch_rows_any(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const RzGroupPieces &pieces, const void *rows, const void *copies,
                     const float *bias, void *out)
 {
-    if (plan.rb == 2) return launch_rows<OP, 2, 2, 256>(c, pieces, rows, copies, bias, out);
+    if (plan.rb == 2 && plan.nc == 256) return launch_rows<OP, 2, 2, 256>(c, pieces, rows, copies, bias, out);
+    if (plan.rb == 2) return launch_rows<OP, 2, 2, 128>(c, pieces, rows, copies, bias, out);
     if (plan.ctas == 2) return launch_rows<OP, 2, 1, 256>(c, pieces, rows, copies, bias, out);
     if (plan.nc == 256) return launch_rows<OP, 1, 1, 256>(c, pieces, rows, copies, bias, out);
-    if (plan.nc == 64) return launch_rows<OP, 1, 1, 64>(c, pieces, rows, copies, bias, out);
-    return launch_rows<OP, 1, 1, 32>(c, pieces, rows, copies, bias, out);
+    return launch_rows<OP, 1, 1, 64>(c, pieces, rows, copies, bias, out);
 }
 
-// Block shape of a bf16 product by an estimate of its time: waves of blocks over the SMs, times a block's stages at the slower of
-// fetching its operands (about 50 bytes a clock and SM) and multiplying them (8192 flops).
+// Block shape of a bf16 product by an estimate of its time: waves of blocks over the SMs, times a block's stages at what a stage of
+// the shape takes (clocks, `fixed` + `per_row` * rows of the block: fits to the cases measured in rz_tc_rows.cuh), plus what a block
+// costs besides.  The host knows the rows and the groups but not how the rows are spread: it reckons with groups of the mean size
+// that end half a piece late.
 RzTcGroupPlan rows_plan(const rz_problem *pb, int groups, int op)
 {
     static const struct {
         int ctas, rb, nmax;
-    } shapes[] = {{2, 2, 256}, {2, 1, 256}, {1, 1, 256}, {1, 1, 64}, {1, 1, 32}};
+        double fixed, per_row;
+    } shapes[] = {{2, 2, 256, 1140.0, 2.4}, {2, 1, 256, 650.0, 1.0}, {1, 1, 256, 700.0, 1.2}, {2, 2, 128, 1140.0, 2.4}, {1, 1, 64, 700.0, 1.2}};
     const double used = (double)(pb->M < groups ? pb->M : groups), mean = (double)pb->M / used;
     const int64_t cols = op == RZ_OP_FORWARD ? pb->N : pb->K;
     const double stages = (double)(((op == RZ_OP_FORWARD ? pb->K : pb->N) + 63) / 64);
@@ -164,15 +167,14 @@ RzTcGroupPlan rows_plan(const rz_problem *pb, int groups, int op)
     double best_time = -1.0;
     for (int i = 0; i < 5; ++i) {
         const auto &s = shapes[i];
-        const double pieces = (double)(int64_t)((mean + s.nmax - 1) / s.nmax), rows = mean / pieces;
-        const double width = (double)((int64_t)((rows + 16 * s.ctas - 1) / (16 * s.ctas)) * 16 * s.ctas);
-        const double fetch = (s.rb * 16384.0 + width / s.ctas * 128.0) / 50.0, multiply = 2.0 * width * s.rb;
-        // a block's clocks; two row blocks do not overlap their epilogue with the next block
-        const double block = stages * (fetch > multiply ? fetch : multiply) + (s.rb == 2 ? 5000.0 : 1500.0);
+        double pieces = mean / s.nmax + 0.5;
+        if (pieces < 1.0) pieces = 1.0;
         const double items = used * pieces * (double)((cols + 128 * s.ctas * s.rb - 1) / (128 * s.ctas * s.rb));
         double waves = items * s.ctas / sms;
         waves = waves < 1.0 ? 1.0 : waves + 0.5;               // half a wave is lost at the end
-        const double time = waves * block;
+        // (accumulators that fill TMEM: the epilogue does not overlap the next block)
+        const double besides = s.rb * s.nmax > 256 ? 10000.0 : 4000.0;
+        const double time = waves * (stages * (s.fixed + s.per_row * mean / pieces) + besides);
         if (best_time < 0.0 || time < best_time || i == forced) {
             best_time = i == forced ? 0.0 : time;
             best.ctas = s.ctas, best.rb = s.rb, best.nc = s.nmax, best.ew = 1, best.step = (uint32_t)s.nmax, best.even = true;

@@ -5,10 +5,13 @@
 // the group has rows and no group pays for a row block it does not fill.  A group with more rows than a block takes is cut into
 // equal pieces (the plan kernel's list).  For few rows a stage is nearly all weight: the kernel then streams weights at the rate the
 // TMA unit fetches them, which is what bounds it.
-//   RB = 1: 128 weight columns a CTA, accumulators double-buffered in TMEM.  RB = 2: 2 x 128, which share the rows' tile (bytes fetched
-//   per flop are what bounds blocks of many rows); both halves of TMEM are then one block's.
+//   RB = 1: 128 weight columns a CTA, accumulators double-buffered in TMEM.  RB = 2: 2 x 128, which share the rows' tile; with NMAX = 256
+//   all of TMEM is then one block's.
 //   CTAS = 2: a cluster of two CTAs drives M = 256 MMAs, each CTA staging its own weight columns and half of the rows.
 //   NMAX: most rows of a block.  Few rows leave the shared memory to a deeper ring.
+// What a stage costs, measured with all weights in L2: a row of a weight box starts at a multiple of
+// 16 bytes and so covers two cache lines, about 4.5 clocks of the TMA unit; an aligned row of X costs 1.8.  A stage of 128 weight
+// columns takes 650 clocks plus one for each row of X, a stage of 2 x 128 takes 1140 plus 2.4.
 // Roles, ring, bounded waits and hash tables of the producers are those of rz_tc_kernel.cuh, except that four warps produce.  Accumulator rows are weight columns, so
 // an epilogue thread owns one output column of 32 rows: bias is one value a thread, and 32 rows x 32 columns are transposed by
 // 2-byte stores into a tile of 64-byte rows (a warp's lanes are neighbours in the row: no bank conflicts), which a bulk tensor
@@ -76,7 +79,8 @@ __device__ __forceinline__ void rows_wait_cycles(uint32_t bar, uint32_t parity, 
 template <int OP, int CTAS, int RB, int NMAX>
 __global__ void __launch_bounds__(rows_threads(RB), 1)
 rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapR16,
-                  const __grid_constant__ CUtensorMap mapR64, const __grid_constant__ CUtensorMap mapRAll, const __grid_constant__ CUtensorMap mapC, const TcRowsParams p)
+                  const __grid_constant__ CUtensorMap mapR64, const __grid_constant__ CUtensorMap mapRAll,
+                  const __grid_constant__ CUtensorMap mapC, const TcRowsParams p)
 {
     constexpr int KC = 64;                                    // contraction elements per stage: one 128-byte row
     constexpr int STAGES = rows_stages(CTAS, RB, NMAX);
@@ -144,16 +148,23 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
     const uint32_t items = pieces * p.tiles_c;
     uint32_t group = 0, row = 0, row_end = 0, width = 0, tc = 0;   // the block decoded last; width = its rows, as the MMA's N
     // blocks are taken in groups of p.group_pieces pieces, column block after column block: the pieces of one group, which read the
-    // same weights, run side by side
-    auto decode = [&](uint32_t item) {
+    // same weights, run side by side.  The next block's piece is fetched while this one is worked on.
+    uint4 ahead = make_uint4(0, 0, 0, 0);
+    uint32_t ahead_tc = 0;
+    auto fetch = [&](uint32_t item) {
+        if (item >= items) return;
         const uint32_t per_group = p.group_pieces * p.tiles_c;
         const uint32_t g = item / per_group, within = item - g * per_group;
         const uint32_t first = g * p.group_pieces, n = min(pieces - first, p.group_pieces);
-        tc = within / n;
-        const uint4 e = __ldg(p.entries + first + (within - tc * n));
-        group = e.x, row = e.y, row_end = e.z;
-        width = (row_end - row + N_STEP - 1) / N_STEP * N_STEP;
+        ahead_tc = within / n;
+        ahead = __ldg(p.entries + first + (within - ahead_tc * n));
     };
+    auto decode = [&](uint32_t item) {   // the items of one role in their order
+        tc = ahead_tc, group = ahead.x, row = ahead.y, row_end = ahead.z;
+        width = (row_end - row + N_STEP - 1) / N_STEP * N_STEP;
+        fetch(item + item_stride);
+    };
+    fetch(first_item);
 
     if (warp == 0 || warp >= 2 + EPI_WARPS) {
         // ===================== producers (both CTAs of a pair) =====================
