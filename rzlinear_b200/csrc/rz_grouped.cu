@@ -159,7 +159,7 @@ rz_group_plan_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
 
 // ---- workspace: lists (header, pieces), tensor maps -----------------------------------------------------------------------------
 constexpr uint32_t SIMT_ROWS = 64, SIMT_CHUNK = 2048;   // rows of an FMA block; rows one block of the FMA weight gradient sums
-constexpr uint32_t PREPARE_ROWS = 64;                   // rows a block of the bias pass sums
+constexpr uint32_t PREPARE_ROWS = 32;                   // rows a block of the bias pass sums
 
 uint32_t most_pieces(const rz_problem *pb, int groups, uint32_t step) { return (uint32_t)(pb->M / step) + (uint32_t)groups; }
 
@@ -257,7 +257,7 @@ rz_grouped_prepare_kernel(const T *__restrict__ dY, const T *__restrict__ Y, T *
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t r = piece.y; r < piece.z; ++r) {
         const size_t at = (size_t)r * N + col;
         Pack g = *reinterpret_cast<const Pack *>(dY + at);

@@ -224,7 +224,7 @@ int launch(const RzLaunchCtx &c, const CUtensorMap &mapA, const CUtensorMap &map
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a_major << 15) | (b_major << 16) | ((uint32_t)(NC >> 3) << 17) |
               ((uint32_t)(PAIR_R >> 4) << 24);
 
-    constexpr int THREADS = num_threads(RB, SPLIT, EW);
+    constexpr int THREADS = num_threads(RB, SPLIT, EW) + 32 * (num_producers(OP, SPLIT, 1) - 1);
     int slots = 0;
     st = resident<rz_tc_kernel<OP, TF32, CTAS, RB, SPLIT, NC, EW, 1>, CTAS>(pb, THREADS, SMEM_TOTAL, &slots);
     if (st) return st;

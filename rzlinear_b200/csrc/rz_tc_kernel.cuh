@@ -130,8 +130,12 @@ __device__ __forceinline__ void wait_cycles(uint32_t bar, uint32_t parity, long 
         if (clock64() - t0 > cycles) break;
 }
 
+// Producer warps: one thread takes longer to issue a weight-gradient stage's four loads (some 800 clocks) than the tensor core to
+// multiply them; the grouped weight gradient has two, which take the stages in turn.
+__host__ __device__ constexpr int num_producers(int op, int split, int grouped) { return op == OP_DW && grouped && !split ? 2 : 1; }
+
 template <int OP, bool TF32, int CTAS, int RB, int SPLIT, int NC, int EW, int GROUPED = 0>
-__global__ void __launch_bounds__(num_threads(RB, SPLIT, EW), 1)
+__global__ void __launch_bounds__(num_threads(RB, SPLIT, EW) + 32 * (num_producers(OP, SPLIT, GROUPED) - 1), 1)
 rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
              const __grid_constant__ CUtensorMap mapC,
              const std::conditional_t<GROUPED != 0, TcGroupParams, TcParams> p)
@@ -304,8 +308,10 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
         return 0u;
     };
 
-    if (warp == 0) {
+    constexpr int PRODUCERS = num_producers(OP, SPLIT, GROUPED);
+    if (warp == 0 || (PRODUCERS == 2 && warp == 2 + EPI_WARPS)) {
         // ===================== producer (both CTAs of a pair) =====================
+        const uint32_t which = PRODUCERS == 2 && warp != 0 ? 1u : 0u;
         uint32_t it = 0;  // stages armed so far
         uint32_t fenced_group = 0xffffffffu;   // (GROUPED DW) group whose maps this thread has acquired
         // transaction bytes of a stage are counted on the leader's barrier
@@ -360,6 +366,7 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
                 if (lane == 0) {
                     for (uint32_t ci = 0; ci < nb; ++ci) {
                         const uint32_t g = it + ci, s = g % STAGES, ph = (g / STAGES) & 1;
+                        if (PRODUCERS == 2 && (g & 1u) != which) continue;
                         if (!mbar_wait_bounded(bar_empty + 8 * s, ph ^ 1, RZ_WAIT_SMEM_EMPTY, p.wait, 2000)) {
                             ok = false;
                             it += ci;
