@@ -665,20 +665,19 @@ int launch_tc(const RzLaunchCtx &c, const CUtensorMap &mapA, const CUtensorMap &
 
     // shared-memory descriptors (bytes)
     const uint32_t atom = KC * 128;
-    const uint32_t mn_kstep = (TF32 ? 8 : 16) * 128;  // contraction rows per MMA x 128-byte rows
     const uint32_t mn_sbo = TF32 ? 512 : 1024;        // tf32 M/N-major: rows group by 4 (32-byte-chunk swizzle)
     const uint32_t mn_layout = TF32 ? 1 : 2;
     p.a_layout = p.b_layout = 2;
     if (OP == OP_FWD) {
-        p.a_lbo = 16, p.a_sbo = 1024, p.a_kstep = 32;             // K-major
-        p.b_lbo = atom, p.b_sbo = mn_sbo, p.b_kstep = mn_kstep;   // N-major
+        p.a_lbo = 16, p.a_sbo = 1024;             // K-major
+        p.b_lbo = atom, p.b_sbo = mn_sbo;   // N-major
         p.b_layout = mn_layout;
     } else if (OP == OP_DX) {
-        p.a_lbo = 16, p.a_sbo = 1024, p.a_kstep = 32;
-        p.b_lbo = 16, p.b_sbo = 1024, p.b_kstep = 32;
+        p.a_lbo = 16, p.a_sbo = 1024;
+        p.b_lbo = 16, p.b_sbo = 1024;
     } else {
-        p.a_lbo = atom, p.a_sbo = mn_sbo, p.a_kstep = mn_kstep;
-        p.b_lbo = atom, p.b_sbo = mn_sbo, p.b_kstep = mn_kstep;
+        p.a_lbo = atom, p.a_sbo = mn_sbo;
+        p.b_lbo = atom, p.b_sbo = mn_sbo;
         p.a_layout = p.b_layout = mn_layout;
     }
     const uint32_t a_major = (OP == OP_DW) ? 1u : 0u, b_major = (OP == OP_DX) ? 0u : 1u;

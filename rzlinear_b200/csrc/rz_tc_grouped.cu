@@ -211,20 +211,22 @@ int launch(const RzLaunchCtx &c, const CUtensorMap &mapA, const CUtensorMap &map
     p.relu = (pb->flags & RZ_FLAG_RELU) ? 1 : 0;
     p.tma_store = 1;
     p.header = pieces.header, p.entries = pieces.entries, p.group_tiles = pieces.group_tiles;
+    // (blocks at the edges hash tiles a little beyond the last group's weight)
+    p.hash32 = rz_hash32(c.hash, (uint64_t)pieces.groups * pieces.group_tiles + 512 / 32, (uint64_t)(pb->N + pb->BN - 1) / pb->BN + 512 / 32);
     int st = rz_wait_context(&p.wait, 2000000000ll);   // also refuses to launch behind a kernel whose wait gave up
     if (st) return st;
 
     // shared-memory descriptors (bytes), as in the ungrouped launches
-    const uint32_t atom = KC * 128, mn_kstep = (TF32 ? 8 : 16) * 128, mn_sbo = TF32 ? 512 : 1024, mn_layout = TF32 ? 1 : 2;
+    const uint32_t atom = KC * 128, mn_sbo = TF32 ? 512 : 1024, mn_layout = TF32 ? 1 : 2;
     p.a_layout = p.b_layout = 2;
-    p.a_lbo = p.b_lbo = 16, p.a_sbo = p.b_sbo = 1024, p.a_kstep = p.b_kstep = 32;   // K-major
-    if (OP != OP_DX) p.b_lbo = atom, p.b_sbo = mn_sbo, p.b_kstep = mn_kstep, p.b_layout = mn_layout;
-    if (OP == OP_DW) p.a_lbo = atom, p.a_sbo = mn_sbo, p.a_kstep = mn_kstep, p.a_layout = mn_layout;
+    p.a_lbo = p.b_lbo = 16, p.a_sbo = p.b_sbo = 1024;   // K-major
+    if (OP != OP_DX) p.b_lbo = atom, p.b_sbo = mn_sbo, p.b_layout = mn_layout;
+    if (OP == OP_DW) p.a_lbo = atom, p.a_sbo = mn_sbo, p.a_layout = mn_layout;
     const uint32_t a_major = OP == OP_DW ? 1u : 0u, b_major = OP == OP_DX ? 0u : 1u, fmt = TF32 ? 2u : 1u;
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a_major << 15) | (b_major << 16) | ((uint32_t)(NC >> 3) << 17) |
               ((uint32_t)(PAIR_R >> 4) << 24);
 
-    constexpr int THREADS = num_threads(RB, SPLIT, EW) + 32 * (num_producers(OP, SPLIT, 1) - 1);
+    constexpr int THREADS = num_threads(RB, SPLIT, EW);
     int slots = 0;
     st = resident<rz_tc_kernel<OP, TF32, CTAS, RB, SPLIT, NC, EW, 1>, CTAS>(pb, THREADS, SMEM_TOTAL, &slots);
     if (st) return st;

@@ -102,7 +102,7 @@ struct TcParams {
     uint32_t br;                // slice rows per B box (FWD: min(BK, stage depth); DX: min(BK, B columns of this CTA))
     uint32_t kparts;            // FWD: B boxes along the contraction per 128-byte column block (stage depth / br)
     uint32_t group_rows;        // row tiles per rasterisation group
-    uint32_t a_lbo, a_sbo, a_kstep, b_lbo, b_sbo, b_kstep;  // descriptor strides, bytes
+    uint32_t a_lbo, a_sbo, b_lbo, b_sbo;                     // descriptor strides, bytes
     uint32_t a_layout, b_layout;                            // descriptor swizzle layout type
     uint32_t idesc;
     float alpha;
@@ -117,6 +117,7 @@ struct TcParams {
 
 // What a grouped launch needs besides; `header` and `entries` are written by the plan kernel before it.
 struct TcGroupParams : TcParams {
+    RzHash32 hash32;
     const uint32_t *header;     // [0] = pieces
     const uint4 *entries;       // {group, first row, end, 0} of each piece
     const CUtensorMap *maps;    // DW: {dY, X} of each group
@@ -130,12 +131,8 @@ __device__ __forceinline__ void wait_cycles(uint32_t bar, uint32_t parity, long 
         if (clock64() - t0 > cycles) break;
 }
 
-// Producer warps: one thread takes longer to issue a weight-gradient stage's four loads (some 800 clocks) than the tensor core to
-// multiply them; the grouped weight gradient has two, which take the stages in turn.
-__host__ __device__ constexpr int num_producers(int op, int split, int grouped) { return op == OP_DW && grouped && !split ? 2 : 1; }
-
 template <int OP, bool TF32, int CTAS, int RB, int SPLIT, int NC, int EW, int GROUPED = 0>
-__global__ void __launch_bounds__(num_threads(RB, SPLIT, EW) + 32 * (num_producers(OP, SPLIT, GROUPED) - 1), 1)
+__global__ void __launch_bounds__(num_threads(RB, SPLIT, EW), 1)
 rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
              const __grid_constant__ CUtensorMap mapC,
              const std::conditional_t<GROUPED != 0, TcGroupParams, TcParams> p)
@@ -308,11 +305,10 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
         return 0u;
     };
 
-    constexpr int PRODUCERS = num_producers(OP, SPLIT, GROUPED);
-    if (warp == 0 || (PRODUCERS == 2 && warp == 2 + EPI_WARPS)) {
+    if (warp == 0) {
         // ===================== producer (both CTAs of a pair) =====================
-        const uint32_t which = PRODUCERS == 2 && warp != 0 ? 1u : 0u;
         uint32_t it = 0;  // stages armed so far
+        uint32_t slot = 0, phase = 1;   // (weight gradient) the ring's next slot, and the parity that says it is free
         uint32_t fenced_group = 0xffffffffu;   // (GROUPED DW) group whose maps this thread has acquired
         // transaction bytes of a stage are counted on the leader's barrier
         uint32_t full_base = bar_full;
@@ -331,9 +327,44 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
                     fenced_group = piece_group;
                 }
             }
+            if constexpr (OP == OP_DW) {
+                // nothing to hash: one thread, with the ring's position and the addresses counted up (a stage's four loads and what is
+                // around them took it 800 clocks with both divided and multiplied out, longer than the stage's MMAs)
+                if (lane == 0) {
+                    int32_t d0 = (int32_t)(c_begin * KC + (GROUPED ? piece_row : 0u));
+#pragma unroll 1
+                    for (uint32_t left = c_end - c_begin; left; --left, d0 += KC) {
+                        if (!mbar_wait_bounded(bar_empty + 8 * slot, phase, RZ_WAIT_SMEM_EMPTY, p.wait, 2000)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t full = full_base + 8 * slot, sa = smem_base + slot * STAGE_BYTES;
+                        if (!PAIR_LOADS) mbar_arrive_expect_tx(bar_full + 8 * slot, LOAD_BYTES);
+                        else if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * slot, LOAD_BYTES * CTAS);
+#pragma unroll
+                        for (int r = 0; r < RB; ++r) {
+#pragma unroll
+                            for (int a = 0; a < A_ATOMS; ++a) {
+                                if (PAIR_LOADS) tma_load_2d_pair(sa + r * A_BLOCK_BYTES + a * ATOM, ma, full, (int32_t)(row0 + r * PAIR_R + a * EPR), d0);
+                                else tma_load_2d(sa + r * A_BLOCK_BYTES + a * ATOM, ma, full, (int32_t)(row0 + r * PAIR_R + a * EPR), d0);
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < B_ATOMS; ++j) {
+                            if (PAIR_LOADS) tma_load_2d_pair(sa + A_BYTES + j * ATOM, mb, full, (int32_t)(col0 + j * EPR), d0);
+                            else tma_load_2d(sa + A_BYTES + j * ATOM, mb, full, (int32_t)(col0 + j * EPR), d0);
+                        }
+                        ++it;
+                        if (++slot == STAGES) slot = 0, phase ^= 1u;
+                    }
+                }
+                __syncwarp();
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                continue;
+            }
             for (uint32_t cb = c_begin; cb < c_end && ok; cb += BATCH) {
                 const uint32_t nb = min((uint32_t)BATCH, c_end - cb);
-                if (OP != OP_DW) {
+                {
                     const uint32_t tps = (OP == OP_FWD) ? (uint32_t)B_ATOMS * p.kparts : (uint32_t)B_COLS / p.br;
                     for (uint32_t e = lane; e < nb * tps; e += 32) {
                         const uint32_t ci = e / tps, j = e - ci * tps;
@@ -366,7 +397,6 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
                 if (lane == 0) {
                     for (uint32_t ci = 0; ci < nb; ++ci) {
                         const uint32_t g = it + ci, s = g % STAGES, ph = (g / STAGES) & 1;
-                        if (PRODUCERS == 2 && (g & 1u) != which) continue;
                         if (!mbar_wait_bounded(bar_empty + 8 * s, ph ^ 1, RZ_WAIT_SMEM_EMPTY, p.wait, 2000)) {
                             ok = false;
                             it += ci;
@@ -379,39 +409,21 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
                         } else {
                             mbar_arrive_expect_tx(bar_full + 8 * s, LOAD_BYTES);
                         }
-                        const uint32_t d0 = (cb + ci) * KC + (GROUPED && OP == OP_DW ? piece_row : 0u);  // contraction start of this stage
-                        if (OP == OP_FWD || OP == OP_DX) {
+                        const uint32_t d0 = (cb + ci) * KC;  // contraction start of this stage
 #pragma unroll
-                            for (int r = 0; r < RB; ++r) {
-                                if (PAIR_LOADS)
-                                    tma_load_2d_pair(sa + r * A_BLOCK_BYTES, &mapA, full, (int32_t)d0, (int32_t)(row0 + r * PAIR_R));
-                                else
-                                    tma_load_2d(sa, &mapA, full, (int32_t)d0, (int32_t)row0);
-                            }
-                            const uint32_t tps = (OP == OP_FWD) ? (uint32_t)B_ATOMS * p.kparts : (uint32_t)B_COLS / p.br;
-                            const uint32_t box_bytes = p.br * 128u;   // (FWD: boxes of one column block are consecutive)
-                            for (uint32_t j = 0; j < tps; ++j) {
-                                const int32_t x = (int32_t)tab_x[ci * MAX_TPS + j], y = (int32_t)tab_y[ci * MAX_TPS + j],
-                                              z = (int32_t)tab_z[ci * MAX_TPS + j];
-                                if (PAIR_LOADS) tma_load_3d_pair(sb + j * box_bytes, &mapB, full, x, y, z);
-                                else tma_load_3d(sb + j * box_bytes, &mapB, full, x, y, z);
-                            }
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < RB; ++r) {
-#pragma unroll
-                                for (int a = 0; a < A_ATOMS; ++a) {
-                                    const uint32_t dst = sa + r * A_BLOCK_BYTES + a * ATOM;
-                                    const int32_t x = (int32_t)(row0 + r * PAIR_R + a * EPR);
-                                    if (PAIR_LOADS) tma_load_2d_pair(dst, ma, full, x, (int32_t)d0);
-                                    else tma_load_2d(dst, ma, full, x, (int32_t)d0);
-                                }
-                            }
-#pragma unroll
-                            for (int j = 0; j < B_ATOMS; ++j) {
-                                if (PAIR_LOADS) tma_load_2d_pair(sb + j * ATOM, mb, full, (int32_t)(col0 + j * EPR), (int32_t)d0);
-                                else tma_load_2d(sb + j * ATOM, mb, full, (int32_t)(col0 + j * EPR), (int32_t)d0);
-                            }
+                        for (int r = 0; r < RB; ++r) {
+                            if (PAIR_LOADS)
+                                tma_load_2d_pair(sa + r * A_BLOCK_BYTES, &mapA, full, (int32_t)d0, (int32_t)(row0 + r * PAIR_R));
+                            else
+                                tma_load_2d(sa, &mapA, full, (int32_t)d0, (int32_t)row0);
+                        }
+                        const uint32_t tps = (OP == OP_FWD) ? (uint32_t)B_ATOMS * p.kparts : (uint32_t)B_COLS / p.br;
+                        const uint32_t box_bytes = p.br * 128u;   // (FWD: boxes of one column block are consecutive)
+                        for (uint32_t j = 0; j < tps; ++j) {
+                            const int32_t x = (int32_t)tab_x[ci * MAX_TPS + j], y = (int32_t)tab_y[ci * MAX_TPS + j],
+                                          z = (int32_t)tab_z[ci * MAX_TPS + j];
+                            if (PAIR_LOADS) tma_load_3d_pair(sb + j * box_bytes, &mapB, full, x, y, z);
+                            else tma_load_3d(sb + j * box_bytes, &mapB, full, x, y, z);
                         }
                     }
                     if (ok) it += nb;
@@ -428,7 +440,18 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
         }
     } else if (warp == 1) {
         // ===================== MMA issuer (leader CTA only) =====================
-        uint32_t it = 0, n_items = 0;
+        // One thread issues everything, instruction after instruction: what does not change from stage to stage is kept out of the
+        // loop (with descriptors built and ring positions divided per MMA, issuing a stage of four MMAs took 800 clocks, more than
+        // the tensor core takes to run them).  A descriptor's low word holds the address in sixteenths, below 2^14: adding to it
+        // cannot carry.
+        constexpr uint32_t MN_KSTEP = (TF32 ? 8 : 16) * 128;   // contraction rows per MMA x 128-byte rows
+        constexpr uint32_t A_KSTEP = OP == OP_DW ? MN_KSTEP : 32, B_KSTEP = OP == OP_DX ? 32 : MN_KSTEP;
+        const uint64_t a0 = make_desc_sw128(smem_base, p.a_lbo, p.a_sbo, p.a_layout);
+        const uint64_t b0 = make_desc_sw128(smem_base + A_BYTES, p.b_lbo, p.b_sbo, p.b_layout);
+        const uint32_t a_lo = (uint32_t)a0, b_lo = (uint32_t)b0;
+        const uint64_t a_hi = a0 >> 32 << 32, b_hi = b0 >> 32 << 32;
+        const uint32_t bar_ready = SPLIT ? bar_split : bar_full;
+        uint32_t n_items = 0, slot = 0, phase = 0;
         for (uint32_t item = cur_begin; item < cur_end && ok && rank == 0; item = next_item, ++n_items) {
             uint32_t tr, tc, c_begin, c_end;
             decode(item, tr, tc, c_begin, c_end);
@@ -439,35 +462,31 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
                 const uint32_t d_tmem = tmem_base + buf * RB * TILE_C;
                 // (CHAINS > 1) stages per main accumulator, and the one in use
                 const uint32_t chain_len = (c_end - c_begin + CHAINS - 1) / CHAINS;
-                uint32_t chain_left = chain_len, chain_col = 0;
-                for (uint32_t c = c_begin; c < c_end && ok; ++c, ++it) {
-                    const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
-                    if (!mbar_wait_bounded((SPLIT ? bar_split : bar_full) + 8 * s, ph, RZ_WAIT_SMEM_FULL, p.wait)) {
+                uint32_t chain_left = chain_len, chain_col = 0, acc = 0, corr_acc = 0;
+#pragma unroll 1
+                for (uint32_t left = c_end - c_begin; left && ok; --left) {
+                    if (!mbar_wait_bounded(bar_ready + 8 * slot, phase, RZ_WAIT_SMEM_FULL, p.wait)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_base + s * STAGE_BYTES, sb = sa + A_BYTES;
-                    bool chain_start = c == c_begin;
+                    const uint32_t al = a_lo + slot * (STAGE_BYTES / 16), bl = b_lo + slot * (STAGE_BYTES / 16);
                     if (CHAINS > 1) {
-                        if (chain_left == 0) chain_left = chain_len, chain_col += NC, chain_start = true;
+                        if (chain_left == 0) chain_left = chain_len, chain_col += NC, acc = 0;
                         --chain_left;
                     }
 #pragma unroll
                     for (int kk = 0; kk < MMAS; ++kk) {
-                        const uint64_t bd = make_desc_sw128(sb + kk * p.b_kstep, p.b_lbo, p.b_sbo, p.b_layout);
-                        const uint32_t acc = (!chain_start || kk > 0) ? 1u : 0u;
-                        const uint32_t corr_acc = (c > c_begin || kk > 0) ? 1u : 0u;
+                        const uint64_t bd = b_hi | (bl + kk * (B_KSTEP / 16));
 #pragma unroll
                         for (int r = 0; r < RB; ++r) {
-                            const uint64_t ad =
-                                make_desc_sw128(sa + r * A_BLOCK_BYTES + kk * p.a_kstep, p.a_lbo, p.a_sbo, p.a_layout);
+                            const uint64_t ad = a_hi | (al + (r * A_BLOCK_BYTES + kk * A_KSTEP) / 16);
                             if (CTAS == 2) tc_mma_pair<TF32>(d_tmem + chain_col + r * TILE_C, ad, bd, p.idesc, acc);
                             else tc_mma<TF32>(d_tmem + chain_col, ad, bd, p.idesc, acc);
                             if (SPLIT) {
                                 // + hi(A) * lo(B) + lo(A) * hi(B)
-                                const uint64_t ad_lo = make_desc_sw128(sa + LOAD_BYTES + kk * p.a_kstep, p.a_lbo, p.a_sbo, p.a_layout);
-                                const uint64_t bd_lo = make_desc_sw128(sb + LOAD_BYTES + kk * p.b_kstep, p.b_lbo, p.b_sbo, p.b_layout);
+                                const uint64_t ad_lo = a_hi | (al + (LOAD_BYTES + kk * A_KSTEP) / 16);
+                                const uint64_t bd_lo = b_hi | (bl + (LOAD_BYTES + kk * B_KSTEP) / 16);
                                 if (CTAS == 2) {
                                     tc_mma_pair<TF32>(d_tmem + CORR_COL, ad, bd_lo, p.idesc, corr_acc);
                                     tc_mma_pair<TF32>(d_tmem + CORR_COL, ad_lo, bd, p.idesc, 1u);
@@ -477,10 +496,12 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
                                 }
                             }
                         }
+                        acc = corr_acc = 1;
                     }
                     // frees this stage in both CTAs once the MMAs have read it
-                    if (CTAS == 2) tc_commit_pair(bar_empty + 8 * s, 3);
-                    else tc_commit(bar_empty + 8 * s);
+                    if (CTAS == 2) tc_commit_pair(bar_empty + 8 * slot, 3);
+                    else tc_commit(bar_empty + 8 * slot);
+                    if (++slot == STAGES) slot = 0, phase ^= 1u;
                 }
                 if (ok) {
                     if (CTAS == 2) tc_commit_pair(bar_tfull + 8 * buf, 3);
@@ -489,7 +510,6 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
             }
             __syncwarp();
             ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-            it = __shfl_sync(0xffffffffu, it, 0);
         }
         if (!ok && lane == 0 && rank == 0) {
             // MMAs may still be running: wait (bounded) until the tensor core has drained
@@ -534,7 +554,8 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
                 if (lane < TILE_C / 32) {
                     const uint32_t kcol = tc * TILE_C + lane * 32, pk = kcol / (uint32_t)p.hash.BK;
                     key_rel = kcol - pk * (uint32_t)p.hash.BK;
-                    key_off = (uint32_t)rz_tile_offset(p.hash, first_tile() + pk, pn);
+                    if constexpr (GROUPED) key_off = rz_tile_offset32(p.hash, p.hash32, first_tile() + pk, pn);
+                    else key_off = (uint32_t)rz_tile_offset(p.hash, pk, pn);
                 }
 #pragma unroll
                 for (int c2 = 0; c2 < TILE_C / 32; ++c2) {
