@@ -31,6 +31,11 @@ def _as(t, dtype, shape=None):
     return t if shape is None or t.shape == shape else t.view(shape)
 
 
+def _operand(t):
+    """t where the kernels can load it 16 bytes at a time; a view that begins elsewhere is copied."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _product(input, hashed_weight, random_numbers, offsets, output_dim, init_factor, config, bias):
     """(output in the compute dtype, int32 offsets, problem, groups, shifted copies): the forward pass and what the backward wants of it."""
     cfg = config if config is not None else DEFAULT_CONFIG
@@ -41,7 +46,7 @@ def _product(input, hashed_weight, random_numbers, offsets, output_dim, init_fac
     groups = off.numel() - 1
     if bias is not None and tuple(bias.shape) != (groups, N):
         raise ValueError(f"bias must have shape {(groups, N)}, got {tuple(bias.shape)}")
-    x = _compute_view(input)
+    x = _operand(_compute_view(input))
     hashed = launchers._hashed_f32(hashed_weight)
     pb = launchers.cached_problem(max(1, M), K, N, H, random_numbers, cfg.block_size_k, cfg.block_size_n, x.dtype,
                                   controls['triton_allow_tf32'], init_factor, cfg.hash_mode, _lib.FLAG_RELU if cfg.relu else 0)
@@ -98,9 +103,9 @@ class RzGroupedLinearFunction(torch.autograd.Function):
     def backward(ctx, grad):
         input, hashed_weight, off, out = ctx.saved_tensors
         pb, groups = ctx.pb, ctx.groups
-        x = _compute_view(input)
+        x = _operand(_compute_view(input))
         M, make = input.shape[0], torch.empty if input.shape[0] else torch.zeros
-        grad = _as(grad, x.dtype).contiguous()
+        grad = _operand(_as(grad, x.dtype).contiguous())
         dx = make((M, pb.K), device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
         dh = make((pb.H,), device=x.device, dtype=torch.float32) if ctx.needs_input_grad[1] else None
         bias_grad = make((groups, pb.N), device=x.device, dtype=torch.float32) if ctx.needs_input_grad[7] else None

@@ -397,3 +397,49 @@ def test_an_expert_model_end_to_end(rz):
     want.backward(g.double())
     for got, exact in ((out.detach(), want.detach()), (w.grad, wd.grad), (up._bias.grad, bd.grad)):
         assert float((got.double() - exact).norm() / exact.norm()) < 5e-5
+
+
+def test_offsets_beyond_32_bits(rz):
+    # 4.6e9 entries of output: rows at the end are computed, stored and differentiated like the first
+    M, K, N, G = 70000, 64, 65536, 2
+    x = torch.randn(M, K, device=DEV).bfloat16()
+    layer = rz.RzGroupedLinear(G, K, N, hashed_weight=torch.nn.Parameter((torch.rand(1 << 20, device=DEV) - 0.5)), bias=False)
+    off = torch.tensor([0, 40, M - 3], device=DEV, dtype=torch.int32)
+    xs = x.clone().requires_grad_()
+    y = layer(xs, off)
+    assert y.numel() > 2**32
+    g = torch.ones((), device=DEV, dtype=BF16).expand(M, N)
+    dx, dh = torch.autograd.grad(y, (xs, layer._hashed_weight), g)
+    sample = torch.tensor([0, 39, 40, 41, M // 2, M - 5, M - 4], device=DEV)
+    few = x[sample].clone().requires_grad_()
+    few_off = torch.tensor([0, 2, 7], device=DEV, dtype=torch.int32)
+    yf = layer(few, few_off)
+    (dxf,) = torch.autograd.grad(yf, few, torch.ones_like(yf))
+    assert float(y[M - 3:].detach().abs().sum()) == 0.0 and float(dx[M - 3:].abs().sum()) == 0.0
+    # the same sums in blocks of other shapes: at most one rounding to bf16 apart
+    assert bool(((y[sample] - yf).detach().float().abs() <= 2.0**-7 * yf.detach().float().abs() + 1e-6).all())
+    assert float((dx[sample] - dxf).float().norm() / dxf.float().norm()) <= 2.0**-7   # (one rounding each)
+    # every word of a group's weight gradient is alpha * (sum over rows of x): check one tile row of group 1 against it
+    want = x[40:M - 3].double().sum(0)
+    words = o.element_index_block(G * K, N, 1 << 20, 32, 64, layer._random_numbers.tolist(), 1, np.arange(G * K), np.arange(N))
+    total = torch.zeros(1 << 20, dtype=torch.float64, device=DEV)
+    w = torch.from_numpy(words).to(DEV)
+    first = x[:40].double().sum(0)
+    total.index_add_(0, w[:K].flatten(), first[:, None].expand(K, N).flatten())
+    total.index_add_(0, w[K:].flatten(), want[:, None].expand(K, N).flatten())
+    assert float((dh.double() - total).norm() / total.norm()) < 1e-5      # the framework's bar for fp32 results
+
+
+def test_views_that_begin_anywhere(rz):
+    case = Case([70, 0, 130, 5], 256, 320, 32, 64, 1, BF16)
+    clean = case.call(rz, 32, 64, 1)
+    for name in ("x", "g"):
+        t = getattr(case, name)
+        buf = torch.empty(t.numel() + 8, device=DEV, dtype=t.dtype)
+        setattr(case, name, buf[3:3 + t.numel()].view(t.shape).copy_(t))
+        assert getattr(case, name).data_ptr() % 16
+    cfg = rz.RzConfig(block_size_k=32, block_size_n=64, hash_mode=1)
+    x = case.x.detach().requires_grad_()
+    y = rz.RzGroupedLinearFunction.apply(x, case.h, torch.tensor(case.R), case.offsets, case.N, case.alpha, cfg)
+    (dx,) = torch.autograd.grad(y, x, case.g)
+    assert torch.equal(y, clean[0]) and torch.equal(dx, clean[1])

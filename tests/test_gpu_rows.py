@@ -70,29 +70,30 @@ def words_of(ids, live, V, D, H, BK, BN, R, mode):
 
 
 CASES = [
-    # tokens, V, D, BK, BN, mode, padding, kind
+    # tokens, V, D, BK, BN, mode, padding, kind;  more than 2^22 entries: tokens are sorted before the gradient
     (1, 1000, 64, 32, 64, 1, None, "text"),
     (1, 33, 1, 4, 3, 0, None, "text"),
     (7, 500, 130, 16, 24, 1, 3, "text"),
     (64, 5000, 256, 32, 32, 0, -1, "even"),
     (255, 128, 63, 32, 64, 1, None, "text"),       # odd row length: no pairs
     (256, 777, 96, 32, 96, 0, None, "one"),
-    (257, 777, 96, 32, 32, 0, 0, "text"),          # first length that is sorted
+    (257, 777, 96, 32, 32, 0, 0, "text"),
     (1000, 50021, 1000, 16, 24, 1, 50020, "text"),
     (2048, 70000, 64, 64, 128, 0, None, "even"),   # row shorter than a hash tile
     (2049, 300, 320, 128, 64, 1, 5, "one"),
-    (8192, 4096, 128, 32, 64, 1, None, "text"),
     (8193, 131072, 72, 64, 64, 0, 7, "outside"),   # rows of no table entry
-    (30000, 65536, 40, 32, 64, 1, None, "text"),
-    (4096, 60000, 4, 32, 4, 1, 9, "even"),         # one chunk, full
-    (12289, 3000, 8, 32, 8, 0, None, "text"),      # a chunk of one token
-    (100000, 40, 2, 4, 2, 0, None, "outside"),     # many chunks, most tokens of no row
-    (16385, 100000, 1024, 32, 64, 1, 5, "text"),   # the longest chunks, and one of one token
-    (6000, 5000, 512, 32, 64, 1, None, "text"),    # four pieces of 64 columns a warp
-    (6000, 5000, 330, 32, 32, 1, 8, "text"),       # the same, halves of a piece apart, a ragged last piece
-    (6000, 900, 450, 16, 96, 0, None, "one"),
-    (5000, 2**31 - 2**13, 64, 2048, 64, 0, None, "outside"),   # the largest ids
     (20000, 2, 50, 1, 50, 0, None, "even"),
+    (5000, 2**31 - 2**13, 64, 2048, 64, 0, None, "outside"),   # the largest ids
+    (257, 3000, 16400, 32, 64, 1, 2, "text"),      # first length that is sorted
+    (2048, 60000, 2052, 32, 32, 1, 9, "even"),     # one chunk, full; a ragged last piece
+    (2049, 3000, 2056, 32, 8, 0, None, "text"),    # a chunk of one token
+    (4097, 5000, 1090, 16, 109, 0, 17, "text"),    # odd segments
+    (6000, 900, 770, 16, 96, 0, None, "one"),      # halves of a piece apart
+    (8193, 131072, 520, 64, 64, 0, 7, "outside"),
+    (16385, 100000, 1024, 32, 64, 1, 5, "text"),   # the longest chunks, and one of one token
+    (70000, 65536, 64, 32, 64, 1, None, "text"),   # many chunks
+    (100000, 40, 47, 4, 2, 0, None, "outside"),    # most tokens of no row
+    (90000, 2, 50, 1, 50, 0, None, "even"),
 ]
 
 
@@ -194,7 +195,7 @@ def test_embedding_types_and_views(rz):
 
 
 def test_embedding_gradient_without_a_plan(rz, rzlib):
-    T, V, D, BK, BN, H = 5000, 300, 128, 32, 64, 9000
+    T, V, D, BK, BN, H = 5000, 300, 1024, 32, 64, 9000
     R = numbers(5, 1)
     ids = torch.randint(0, V, (T,), device=DEV)
     g = torch.ones(T, D, device=DEV)                                               # (sums of ones are exact in any order)
@@ -221,8 +222,9 @@ def test_embedding_empty_and_no_tokens(rz):
     assert float(out.detach().abs().sum()) == 0.0 and float(layer._hashed_weight.grad.abs().sum()) == 0.0
 
 
-def test_embedding_on_another_stream_and_in_a_graph(rz):
-    V, D, T = 2000, 128, 1500
+@pytest.mark.parametrize("T", [1500, 40000])
+def test_embedding_on_another_stream_and_in_a_graph(rz, T):
+    V, D = 2000, 128
     layer = rz.RzEmbedding(V, D).to(DEV)
     w = layer._hashed_weight
     ids = torch.randint(0, V, (T,), device=DEV)
@@ -249,3 +251,20 @@ def test_embedding_on_another_stream_and_in_a_graph(rz):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(held[0], want[0]) and torch.equal(held[1], want[1])
+
+
+def test_embedding_beyond_32_bit_offsets(rz):
+    # 4.3e9 entries of output and gradient: the last rows are looked up, and their gradients added, as the first
+    T, V, D = 33000, 300, 131072
+    assert T * D > 2**32
+    layer = rz.RzEmbedding(V, D, hashed_weight=torch.nn.Parameter(torch.randn(1 << 20, device=DEV)), out_dtype=BF16)
+    ids = torch.randint(0, V, (T,), device=DEV)
+    out = layer(ids)
+    for t in (0, T // 2, T - 2, T - 1):
+        assert torch.equal(out[t], layer(ids[t:t + 1])[0])
+    (whole,) = torch.autograd.grad(out, layer._hashed_weight, torch.ones((), device=DEV, dtype=BF16).expand(T, D))
+    count = torch.bincount(ids, minlength=V)
+    rows = layer(torch.arange(V, device=DEV))
+    (each,) = torch.autograd.grad(rows, layer._hashed_weight, count[:, None].to(BF16).expand(V, D))
+    # counts up to 256 are whole in bf16 and every word's sum is a whole number below 2^24: exact in any order
+    assert int(count.max()) <= 256 and float(whole.max()) < 2**24 and torch.equal(whole, each)

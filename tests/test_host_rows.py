@@ -51,10 +51,11 @@ def test_embedding_refusals(rzlib):
     assert fwd(ids=None) == -1 and fwd(h=None) == -1 and fwd(out=None) == -1
     assert fwd(ids=ctypes.c_void_p((1 << 20) + 4)) == -5 and fwd(out=ctypes.c_void_p((1 << 20) + 2)) == -5
     assert fwd(pb=_pb(rzlib, H=2048)) == -3 and fwd(pb=_pb(rzlib, K=0)) == -2 and fwd(pb=_pb(rzlib, io=1, prec=1)) == -4
-    assert lib.rz_embedding_plan_bytes(ref(_pb(rzlib, M=256))) == 0
-    big = _pb(rzlib, M=257)
+    assert lib.rz_embedding_plan_bytes(ref(_pb(rzlib, M=256, N=1 << 20))) == 0            # too few tokens, too few words: not sorted
+    assert lib.rz_embedding_plan_bytes(ref(_pb(rzlib, M=1 << 12, N=1 << 10))) == 0
+    big = _pb(rzlib, M=1 << 12, N=1025)
     need = lib.rz_embedding_plan_bytes(ref(big))
-    assert need == 257 * 8 and fwd(pb=big, plan=some, pbytes=need - 1) == -11
+    assert need == 4096 * 8 and fwd(pb=big, plan=some, pbytes=need - 1) == -11
     assert fwd(pb=big, plan=ctypes.c_void_p((1 << 20) + 2), pbytes=need) == -5
     assert lib.rz_embedding_backward(ref(big), some, -1, some, some, some, need - 1, None) == -11
     assert lib.rz_embedding_backward(ref(pb), some, -1, some, None, None, 0, None) == -1
