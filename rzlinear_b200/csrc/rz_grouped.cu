@@ -69,6 +69,7 @@ rz_group_plan_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     __shared__ uint32_t first[RZ_GROUPS_MAX + 1];   // pieces before each group
     __shared__ uint32_t warp_sums[32];
     __shared__ __align__(128) CUtensorMap staged[PLAN_THREADS / 32];
+    rzptx::grid_launch_dependents();
     const uint32_t G = p.groups, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     uint32_t carry = 0;

@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "rz_common.h"
+#include "rz_ptx.cuh"
 
 namespace {
 
@@ -250,7 +251,7 @@ rz_embedding_kernel(const int64_t *__restrict__ ids, int64_t padding, const floa
     }
     // a token sort may run beside this kernel: the grid ends after it does.  (One block waits; if all did, the ones not yet
     // started would wait for those that had finished.)
-    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x == 0) rzptx::grid_wait();
 }
 
 // The same for hash tiles and rows of whole 64-word pieces: a unit is 64 words, so every unit is full, its place in the output
@@ -295,7 +296,7 @@ rz_embedding_pieces_kernel(const int64_t *__restrict__ ids, int64_t padding, con
     }
     // a token sort may run beside this kernel: the grid ends after it does.  (One block waits; if all did, the ones not yet
     // started would wait for those that had finished.)
-    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x == 0) rzptx::grid_wait();
 }
 
 // ---- embedding gradient -----------------------------------------------------------------------------------------------
@@ -324,7 +325,7 @@ rz_token_sort_kernel(const int64_t *__restrict__ ids, int64_t padding, uint32_t 
     uint32_t *count = skey + CHUNK;                                               // [CHUNK_WARPS][256]
     uint16_t *spos = reinterpret_cast<uint16_t *>(count + CHUNK_WARPS * 256);     // [CHUNK]
     __shared__ uint32_t warp_sums[32];
-    asm volatile("griddepcontrol.launch_dependents;");   // the lookup runs beside this kernel, and waits for it at its end
+    rzptx::grid_launch_dependents();   // the lookup runs beside this kernel, and waits for it at its end
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1u << width;
     const uint32_t begin = blockIdx.x * CHUNK, valid = min(CHUNK, T - begin);
     const uint32_t first = warp * (32 * ITEMS) + lane;

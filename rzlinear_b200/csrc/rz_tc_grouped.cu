@@ -63,15 +63,18 @@ int launch_persistent(Kernel kernel, int threads, int smem, int slots, uint64_t 
 {
     if (most >= 0x80000000ull) return RZ_ERR_SHAPE;   // block numbers are 32-bit words
     cudaLaunchConfig_t cfg;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     memset(&cfg, 0, sizeof(cfg));
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CTAS, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CTAS, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+    // The kernel sets itself up (barriers, TMEM) beside the one before it, the plan's, and waits for that before it reads anything.
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.blockDim = dim3(threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.gridDim = dim3((unsigned)(most < (uint64_t)slots ? most : (uint64_t)slots) * CTAS, 1, 1);
-    cfg.attrs = attr, cfg.numAttrs = CTAS == 2 ? 1 : 0;
+    cfg.attrs = attr, cfg.numAttrs = CTAS == 2 ? 2 : 1;
     const int st = rz_record_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), "grouped tcgen05 kernel launch");
     rz_count_launch(1);
     if (st) return st;

@@ -245,7 +245,8 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
     uint32_t cur_begin = first_item, cur_end = p.total_items;
     uint32_t tiles_r = p.tiles_r;
     if constexpr (GROUPED) {
-        const uint32_t pieces = __ldg(p.header);
+        grid_wait();   // (up to here: beside the kernel before this one)
+        const uint32_t pieces = ld_behind_wait(p.header);
         if (OP != OP_DW) tiles_r = pieces;
         cur_end = OP == OP_DW ? pieces * p.tiles_r * p.tiles_c : pieces * p.tiles_c;
     }
@@ -259,7 +260,7 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
     auto decode = [&](uint32_t item, uint32_t &tr, uint32_t &tc, uint32_t &c_begin, uint32_t &c_end) {
         if constexpr (GROUPED && OP == OP_DW) {
             const uint32_t per_piece = p.tiles_r * p.tiles_c, piece = item / per_piece;
-            const uint4 e = __ldg(p.entries + piece);
+            const uint4 e = ld_behind_wait(p.entries + piece);
             piece_group = e.x, piece_row = e.y, piece_end = e.z;
             tile = item - piece * per_piece;
             c_begin = 0;
@@ -293,7 +294,7 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
         tr = first_r + within % gsz;
         tc = within / gsz;
         if constexpr (GROUPED && OP != OP_DW) {
-            const uint4 e = __ldg(p.entries + tr);
+            const uint4 e = ld_behind_wait(p.entries + tr);
             piece_group = e.x, piece_row = e.y, piece_end = e.z;
         }
     };

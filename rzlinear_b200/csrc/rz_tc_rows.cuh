@@ -143,8 +143,9 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
 
+    grid_wait();   // (up to here: beside the kernel before this one)
     bool ok = true;
-    const uint32_t pieces = __ldg(p.header);
+    const uint32_t pieces = ld_behind_wait(p.header);
     const uint32_t items = pieces * p.tiles_c;
     uint32_t group = 0, row = 0, row_end = 0, width = 0, tc = 0;   // the block decoded last; width = its rows, as the MMA's N
     // blocks are taken in groups of p.group_pieces pieces, column block after column block: the pieces of one group, which read the
@@ -157,7 +158,7 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
         const uint32_t g = item / per_group, within = item - g * per_group;
         const uint32_t first = g * p.group_pieces, n = min(pieces - first, p.group_pieces);
         ahead_tc = within / n;
-        ahead = __ldg(p.entries + first + (within - ahead_tc * n));
+        ahead = ld_behind_wait(p.entries + first + (within - ahead_tc * n));
     };
     auto decode = [&](uint32_t item) {   // the items of one role in their order
         tc = ahead_tc, group = ahead.x, row = ahead.y, row_end = ahead.z;

@@ -418,7 +418,9 @@ def test_offsets_beyond_32_bits(rz):
     assert float(y[M - 3:].detach().abs().sum()) == 0.0 and float(dx[M - 3:].abs().sum()) == 0.0
     # the same sums in blocks of other shapes: at most one rounding to bf16 apart
     assert bool(((y[sample] - yf).detach().float().abs() <= 2.0**-7 * yf.detach().float().abs() + 1e-6).all())
-    assert float((dx[sample] - dxf).float().norm() / dxf.float().norm()) <= 2.0**-7   # (one rounding each)
+    off_by = (dx[sample] - dxf).float().norm() / dxf.float().norm()
+    bad = ((dx[sample] - dxf).float().abs() > 1.0).nonzero()
+    assert float(off_by) <= 2.0**-7, (bad.shape, bad[:12].tolist(), [(float(dx[sample][i, j]), float(dxf[i, j])) for i, j in bad[:12].tolist()], bool(dx.isfinite().all()), int((~dx.isfinite()).any(1).sum()), (~dx.isfinite()).any(1).nonzero()[:10].flatten().tolist())
     # every word of a group's weight gradient is alpha * (sum over rows of x): check one tile row of group 1 against it
     want = x[40:M - 3].double().sum(0)
     words = o.element_index_block(G * K, N, 1 << 20, 32, 64, layer._random_numbers.tolist(), 1, np.arange(G * K), np.arange(N))
