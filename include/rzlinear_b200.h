@@ -204,8 +204,8 @@ int rz_embedding_forward(const rz_problem *pb, const int64_t *ids, int64_t paddi
 
 /* Its gradient: dH[offset(k / BK, n / BN) + (k % BK) * BN + n % BN] += alpha * (sum of dOut[m, n] over the tokens with
    ids[m] = k), fp32; dH is zeroed first unless RZ_FLAG_ACCUMULATE_DH.  Tokens that gave zeros contribute nothing, whatever
-   their dOut holds.  With the plan that rz_embedding_forward made of the same ids, K and padding_idx, the rows of equal tokens are
-   summed before they are added into dH; without one (NULL) every token's row is added by itself, which is right and, where tokens
+   their dOut holds.  With the plan that rz_embedding_forward made for the same problem, ids and padding_idx, the rows of equal tokens
+   are summed before they are added into dH; without one (NULL) every token's row is added by itself, which is right and, where tokens
    repeat, slow.  The additions are fp32 reductions whose order is not fixed, as in rz_linear_backward_weight. */
 int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padding_idx, const void *dOut, float *dH,
                           const void *plan, size_t plan_bytes, void *stream);

@@ -379,6 +379,7 @@ int rz_grouped_forward(const rz_problem *pb, int64_t groups, const int32_t *offs
     if (st) return st;
     const bool tc = use_tc_grouped(pb);
     if (!X || !Y || (tc ? !copies : !hashed)) return RZ_ERR_NULL;
+    if (!aligned_to(hashed, 4) || !aligned_to(bias, 4)) return RZ_ERR_ALIGN;
     st = check_grouped(pb, groups, offsets, X, Y, copies, copies_bytes, workspace, workspace_bytes, tc, true);
     if (st) return st;
     return rz_grouped_run_forward(make_ctx(pb, stream), (int)groups, offsets, X, hashed, copies, bias, Y, workspace, tc);
@@ -393,7 +394,7 @@ int rz_grouped_backward(const rz_problem *pb, int64_t groups, const int32_t *off
     const bool tc = use_tc_grouped(pb);
     if (!dY || (dH && !X) || (dX && (tc ? !copies : !hashed)) || (Y && !dYm) || !(bias_grad || dX || dH)) return RZ_ERR_NULL;
     const uintptr_t element = pb->io_dtype == RZ_BF16 ? 2 : 4;
-    if (!aligned_to(dH, 4) || !aligned_to(bias_grad, 4) || !aligned_to(Y, element) || !aligned_to(dYm, tc ? 16 : element) ||
+    if (!aligned_to(dH, 4) || !aligned_to(bias_grad, 4) || !aligned_to(hashed, 4) || !aligned_to(Y, element) || !aligned_to(dYm, tc ? 16 : element) ||
         !aligned_to(X, dH && tc ? 16 : element))
         return RZ_ERR_ALIGN;
     st = check_grouped(pb, groups, offsets, dY, dX, copies, copies_bytes, workspace, workspace_bytes, tc, dX != nullptr);

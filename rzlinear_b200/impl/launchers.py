@@ -110,24 +110,29 @@ def cached_shadow(pb, hashed_weight: torch.Tensor, hashed_f32: torch.Tensor, nby
         version, ptr = hashed_weight._version, hashed_weight.data_ptr()
     except RuntimeError:            # inference tensors keep no version counter: nothing to key a cache on
         return alloc_shadow(pb, hashed_f32)
-    stream = _lib._stream(hashed_f32.device)
+    device = hashed_f32.device
+    stream = _lib._stream(device)
     if torch.cuda.is_current_stream_capturing():
         # a buffer from the graph's own memory pool, filled by a node of the graph; the eager cache is left alone
-        shadow = torch.empty(nbytes, dtype=torch.uint8, device=hashed_f32.device)
+        shadow = torch.empty(nbytes, dtype=torch.uint8, device=device)
         _lib.shadow_refresh(pb, hashed_f32, shadow)
         return shadow
     entry = cache.get(key)
-    if entry is not None and entry["shadow"].numel() >= nbytes and entry["shadow"].device == hashed_f32.device:
+    if entry is not None and entry["shadow"].numel() >= nbytes and entry["shadow"].device == device:
+        shadow = entry["shadow"]
+        if entry["stream"] != stream:
+            # nobody outside knows of this buffer: when it goes (with the weight, or for a larger one) its memory waits for this stream too
+            shadow.record_stream(torch.cuda.current_stream(device))
         if entry["version"] == version and entry["ptr"] == ptr:
             if entry["stream"] != stream:
-                torch.cuda.current_stream(hashed_f32.device).wait_event(entry["filled"])    # the refresh ran on another stream
-            return entry["shadow"]
-        shadow = entry["shadow"]                      # same buffer, new contents
+                torch.cuda.current_stream(device).wait_event(entry["filled"])    # the refresh ran on another stream
+            return shadow
+        # else: same buffer, new contents
     else:
-        shadow = torch.empty(nbytes, dtype=torch.uint8, device=hashed_f32.device)
+        shadow = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _lib.shadow_refresh(pb, hashed_f32, shadow)
     filled = torch.cuda.Event()
-    filled.record(torch.cuda.current_stream(hashed_f32.device))
+    filled.record(torch.cuda.current_stream(device))
     cache[key] = {"version": version, "ptr": ptr, "shadow": shadow, "stream": stream, "filled": filled}
     return shadow
 

@@ -350,6 +350,34 @@ def test_two_streams_and_a_graph(rz):
         assert torch.equal(held[0], fresh[0]) and torch.equal(held[1], fresh[1])
 
 
+def test_copies_replaced_while_another_stream_reads_them(rz):
+    # a linear layer over the same array wants a larger buffer than a grouped call: the smaller one, still read by a call that waits on
+    # another stream, must not be handed out again before that call has run
+    case = Case([200, 0, 90], 256, 512, 32, 64, 1, BF16)
+    cfg = rz.RzConfig(block_size_k=32, block_size_n=64, hash_mode=1)
+    R, h = torch.tensor(case.R), case.h.clone()
+    grouped = lambda: rz.RzGroupedLinearFunction.apply(case.x, h, R, case.offsets, case.N, case.alpha, cfg)
+    want = grouped()
+    before = h._rz_shadow_cache[next(iter(h._rz_shadow_cache))]["shadow"].numel()
+    wide = torch.randn(64, 1024, device=DEV).bfloat16()
+    linear = lambda weight: rz.RzLinearFunction.apply(wide, weight, R, 4096, 0, case.alpha, cfg)
+    fill = lambda: torch.full((before,), 0x7f, dtype=torch.uint8, device=DEV)
+    linear(h.clone()), fill()                  # (load their kernels, which would wait for the device later)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grouped()                              # (gets this stream its memory)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)         # some 0.1 s
+        got = grouped()
+    linear(h)
+    entry, = h._rz_shadow_cache.values()
+    assert entry["shadow"].numel() > before    # replaced
+    garbage = [fill() for _ in range(16)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and len(garbage) == 16
+
 def test_an_expert_model_end_to_end(rz):
     # tokens -> table -> rows sorted by expert -> two grouped products -> weighted sum per token, forward and backward, all weights
     # slices of one hashed array; against the same model with materialised weights in 64 bits.  Five products deep, each within the
@@ -418,9 +446,7 @@ def test_offsets_beyond_32_bits(rz):
     assert float(y[M - 3:].detach().abs().sum()) == 0.0 and float(dx[M - 3:].abs().sum()) == 0.0
     # the same sums in blocks of other shapes: at most one rounding to bf16 apart
     assert bool(((y[sample] - yf).detach().float().abs() <= 2.0**-7 * yf.detach().float().abs() + 1e-6).all())
-    off_by = (dx[sample] - dxf).float().norm() / dxf.float().norm()
-    bad = ((dx[sample] - dxf).float().abs() > 1.0).nonzero()
-    assert float(off_by) <= 2.0**-7, (bad.shape, bad[:12].tolist(), [(float(dx[sample][i, j]), float(dxf[i, j])) for i, j in bad[:12].tolist()], bool(dx.isfinite().all()), int((~dx.isfinite()).any(1).sum()), (~dx.isfinite()).any(1).nonzero()[:10].flatten().tolist())
+    assert float((dx[sample] - dxf).float().norm() / dxf.float().norm()) <= 2.0**-7
     # every word of a group's weight gradient is alpha * (sum over rows of x): check one tile row of group 1 against it
     want = x[40:M - 3].double().sum(0)
     words = o.element_index_block(G * K, N, 1 << 20, 32, 64, layer._random_numbers.tolist(), 1, np.arange(G * K), np.arange(N))

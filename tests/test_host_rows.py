@@ -111,12 +111,17 @@ def test_grouped_refusals(rzlib):
     assert fwd(cb=copies - 1) == -11 and fwd(wb=ws - 1) == -11
     assert fwd(x=odd) == -5 and fwd(y=odd) == -5 and fwd(w=odd) == -5 and fwd(off=ctypes.c_void_p((1 << 20) + 2)) == -5
 
+    half = ctypes.c_void_p((1 << 20) + 2)                                               # bias and hashed array: whole floats
+    assert fwd(h=half) == -5
+    assert lib.rz_grouped_forward(ref(pb), 4, some, some, some, some, copies, half, some, some, ws, None) == -5
+
     def bwd(x=some, dy=some, y=None, h=some, c=some, dym=None, db=None, dx=some, dh=some, w=some, wb=ws):
         return lib.rz_grouped_backward(ref(pb), 4, some, x, dy, y, h, c, copies, dym, db, dx, dh, w, wb, None)
 
     assert bwd(dy=None) == -1 and bwd(x=None) == -1 and bwd(c=None) == -1 and bwd(dx=None, dh=None) == -1 and bwd(w=None) == -1
     assert bwd(y=some) == -1                                                            # a mask, and nowhere to put the masked gradient
     assert bwd(wb=ws - 1) == -11 and bwd(dy=odd) == -5 and bwd(x=odd) == -5 and bwd(dx=odd) == -5 and bwd(y=some, dym=odd) == -5
+    assert bwd(h=half) == -5 and bwd(db=half) == -5 and bwd(dh=half) == -5
 
     layer = rz.RzGroupedLinear(4, 128, 64)
     assert layer._hashed_weight.shape == (2048,) and layer._bias.shape == (4, 64)
