@@ -343,9 +343,9 @@ int rz_grouped_run_backward(const RzLaunchCtx &c, int groups, const int32_t *off
         if (tc) {   // A = dY, B = X, boxes of one 128-byte row by a stage's contraction rows
             const rztc::Geometry g = rztc::geometry(pb);
             const bool tf32 = pb->precision != RZ_PREC_BF16;
-            st = rztc::map_matrix(&plan.mapA, tf32, true, grad, pb->M, pb->N, g.epr, g.epr);
+            st = rztc::map_matrix(&plan.mapA, tf32, true, grad, pb->M, pb->N, g.epr, g.epr, false);
             if (st) return st;
-            st = rztc::map_matrix(&plan.mapB, tf32, true, X, pb->M, pb->K, g.epr, g.epr);
+            st = rztc::map_matrix(&plan.mapB, tf32, true, X, pb->M, pb->K, g.epr, g.epr, false);
             if (st) return st;
             maps = plan.add_maps();
         }

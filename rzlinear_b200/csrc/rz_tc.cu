@@ -306,7 +306,7 @@ struct MapCache {
 namespace rztc {
 
 int encode(CUtensorMap *map, bool tf32, int mn_major, void *base, int rank, const uint64_t *dims,
-           const uint64_t *strides_bytes, const uint32_t *box)
+           const uint64_t *strides_bytes, const uint32_t *box, bool keep)
 {
     static thread_local MapCache cache;
     MapKey k;
@@ -314,7 +314,7 @@ int encode(CUtensorMap *map, bool tf32, int mn_major, void *base, int rank, cons
     k.base = base, k.rank = rank, k.tf32 = tf32, k.mn_major = mn_major;
     for (int i = 0; i < rank; ++i) k.dims[i] = dims[i], k.box[i] = box[i];
     for (int i = 0; i + 1 < rank; ++i) k.strides[i] = strides_bytes[i];
-    for (int i = 0; i < cache.used; ++i)
+    for (int i = 0; keep && i < cache.used; ++i)
         if (cache.key[i] == k) {
             *map = cache.map[i];
             return RZ_OK;
@@ -349,6 +349,7 @@ int encode(CUtensorMap *map, bool tf32, int mn_major, void *base, int rank, cons
         snprintf(msg, sizeof(msg), "cuTensorMapEncodeTiled failed (CUresult %d, rank %d)", (int)r, rank);
         return rz_record_cuda(cudaErrorInvalidValue, msg);
     }
+    if (!keep) return RZ_OK;
     const int slot = cache.used < MapCache::N ? cache.used++ : (cache.next = (cache.next + 1) % MapCache::N);
     cache.key[slot] = k;
     cache.map[slot] = *map;
@@ -782,24 +783,24 @@ int forced_shape()
 
 // 2-D map over a row-major matrix [rows][cols] of the operand type
 int map_matrix(CUtensorMap *map, bool tf32, int mn_major, const void *base, uint64_t rows, uint64_t cols,
-               uint32_t box_cols, uint32_t box_rows)
+               uint32_t box_cols, uint32_t box_rows, bool keep)
 {
     const int es = tf32 ? 4 : 2;
     uint64_t dims[2] = {cols, rows};
     uint64_t strides[1] = {cols * (uint64_t)es};
     uint32_t box[2] = {box_cols, box_rows};
-    return encode(map, tf32, mn_major, const_cast<void *>(base), 2, dims, strides, box);
+    return encode(map, tf32, mn_major, const_cast<void *>(base), 2, dims, strides, box, keep);
 }
 
 // 3-D map over the shadow: {element of a copy, slice row (stride BN elements), copy}
-int map_shadow(CUtensorMap *map, const rz_problem *pb, bool mn_major, const void *shadow, uint32_t box_rows)
+int map_shadow(CUtensorMap *map, const rz_problem *pb, bool mn_major, const void *shadow, uint32_t box_rows, bool keep)
 {
     const Geometry g = geometry(pb);
     const bool tf32 = pb->precision != RZ_PREC_BF16;
     uint64_t dims[3] = {g.Hc, (uint64_t)pb->BK, (uint64_t)g.ns};
     uint64_t strides[2] = {(uint64_t)pb->BN * g.es, (uint64_t)g.copy_stride};
     uint32_t box[3] = {(uint32_t)g.epr, box_rows, 1};
-    return encode(map, tf32, mn_major, const_cast<void *>(shadow), 3, dims, strides, box);
+    return encode(map, tf32, mn_major, const_cast<void *>(shadow), 3, dims, strides, box, keep);
 }
 
 }  // namespace rztc

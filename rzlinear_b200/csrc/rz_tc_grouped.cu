@@ -122,15 +122,15 @@ int launch_rows(const RzLaunchCtx &c, const RzGroupPieces &pieces, const void *r
     int st = rz_wait_context(&p.wait, 2000000000ll);   // also refuses to launch behind a kernel whose wait gave up
     if (st) return st;
     CUtensorMap mapW, mapR16, mapR64, mapRAll, mapC;
-    st = map_shadow(&mapW, pb, OP == ROWS_FWD, copies, 1u << p.br_log2);
+    st = map_shadow(&mapW, pb, OP == ROWS_FWD, copies, 1u << p.br_log2, false);
     if (st) return st;
-    st = map_matrix(&mapR16, false, 0, rows, pb->M, depth, 64, 16);
+    st = map_matrix(&mapR16, false, 0, rows, pb->M, depth, 64, 16, false);
     if (st) return st;
-    st = map_matrix(&mapR64, false, 0, rows, pb->M, depth, 64, 64);
+    st = map_matrix(&mapR64, false, 0, rows, pb->M, depth, 64, 64, false);
     if (st) return st;
-    st = map_matrix(&mapRAll, false, 0, rows, pb->M, depth, 64, NMAX / CTAS);
+    st = map_matrix(&mapRAll, false, 0, rows, pb->M, depth, 64, NMAX / CTAS, false);
     if (st) return st;
-    st = map_matrix(&mapC, false, PLAIN_LAYOUT, out, pb->M, cols, 32, 32);
+    st = map_matrix(&mapC, false, PLAIN_LAYOUT, out, pb->M, cols, 32, 32, false);
     if (st) return st;
     constexpr int SMEM = rows_smem_total(CTAS, RB, NMAX), THREADS = rows_threads(RB);
     static_assert(SMEM <= ROWS_SMEM_LIMIT, "shared memory budget");
@@ -330,11 +330,11 @@ int rz_tc_grouped_forward(const RzLaunchCtx &c, const RzTcGroupPlan &plan, const
     p.bias = bias;
     p.out = Y;
     CUtensorMap mapA, mapB, mapC;
-    int st = map_matrix(&mapA, true, 0, X, pb->M, pb->K, g.epr, TILE_R);
+    int st = map_matrix(&mapA, true, 0, X, pb->M, pb->K, g.epr, TILE_R, false);
     if (st) return st;
-    st = map_shadow(&mapB, pb, true, copies, pb->BK < g.epr ? pb->BK : g.epr);
+    st = map_shadow(&mapB, pb, true, copies, pb->BK < g.epr ? pb->BK : g.epr, false);
     if (st) return st;
-    st = map_matrix(&mapC, true, 0, Y, pb->M, pb->N, g.epr, 32);
+    st = map_matrix(&mapC, true, 0, Y, pb->M, pb->N, g.epr, 32, false);
     if (st) return st;
     return launch_any<OP_FWD>(c, plan, mapA, mapB, mapC, p, pieces);
 }
@@ -349,12 +349,12 @@ int rz_tc_grouped_backward_input(const RzLaunchCtx &c, const RzTcGroupPlan &plan
     memset(&p, 0, sizeof(p));
     p.out = dX;
     CUtensorMap mapA, mapB, mapC;
-    int st = map_matrix(&mapA, true, 0, dY, pb->M, pb->N, g.epr, TILE_R);
+    int st = map_matrix(&mapA, true, 0, dY, pb->M, pb->N, g.epr, TILE_R, false);
     if (st) return st;
     const uint32_t bcols = (uint32_t)(plan.nc / plan.ctas);
-    st = map_shadow(&mapB, pb, false, copies, (uint32_t)pb->BK < bcols ? (uint32_t)pb->BK : bcols);
+    st = map_shadow(&mapB, pb, false, copies, (uint32_t)pb->BK < bcols ? (uint32_t)pb->BK : bcols, false);
     if (st) return st;
-    st = map_matrix(&mapC, true, 0, dX, pb->M, pb->K, g.epr, 32);
+    st = map_matrix(&mapC, true, 0, dX, pb->M, pb->K, g.epr, 32, false);
     if (st) return st;
     return launch_any<OP_DX>(c, plan, mapA, mapB, mapC, p, pieces);
 }

@@ -25,16 +25,16 @@ inline Geometry geometry(const rz_problem *pb)
     return g;
 }
 
-// Tensor maps, kept per host thread for calls that repeat.
+// Tensor maps.  `keep`: the host thread remembers the last few it made, for calls that repeat with the same buffers.
 // `mn_major`: 0 = K-major operand, 1 = M/N-major, PLAIN_LAYOUT = rows one behind the other without a swizzle
 constexpr int PLAIN_LAYOUT = 2;
 int encode(CUtensorMap *map, bool tf32, int mn_major, void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
-           const uint32_t *box);
+           const uint32_t *box, bool keep);
 // 2-D map over a row-major matrix [rows][cols] of the operand type
 int map_matrix(CUtensorMap *map, bool tf32, int mn_major, const void *base, uint64_t rows, uint64_t cols, uint32_t box_cols,
-               uint32_t box_rows);
+               uint32_t box_rows, bool keep = true);
 // 3-D map over the shadow: {element of a copy, slice row (stride BN elements), copy}
-int map_shadow(CUtensorMap *map, const rz_problem *pb, bool mn_major, const void *shadow, uint32_t box_rows);
+int map_shadow(CUtensorMap *map, const rz_problem *pb, bool mn_major, const void *shadow, uint32_t box_rows, bool keep = true);
 int num_sms();
 // Block shape that RZ_TC_CONFIG forces, counted from the largest (0 = pair 512 x 256 .. 4 = 128 x 64), or -1
 int forced_shape();
