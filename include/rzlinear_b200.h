@@ -226,7 +226,8 @@ int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padd
 size_t rz_grouped_copies_bytes(const rz_problem *pb);
 size_t rz_grouped_workspace_bytes(const rz_problem *pb, int64_t groups);
 
-/* Y[r,:] = alpha * X[r,:] . W_g (+ bias[g,:], fp32 [groups, N], may be NULL) (+ ReLU with RZ_FLAG_RELU) for r in group g. */
+/* Y[r,:] = alpha * X[r,:] . W_g (+ bias[g,:], fp32 [groups, N], may be NULL) (+ ReLU with RZ_FLAG_RELU, which lets a NaN through) for r in
+   group g.  fp32 precision on the tensor cores: an infinite operand gives NaN. */
 int rz_grouped_forward(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const float *hashed,
                        const void *copies, size_t copies_bytes, const float *bias, void *Y, void *workspace, size_t workspace_bytes,
                        void *stream);
@@ -236,7 +237,7 @@ int rz_grouped_forward(const rz_problem *pb, int64_t groups, const int32_t *offs
      dH[word of W_g[k,n]] += alpha * sum over the rows r of group g of X[r,k] dY[r,n], for every group, zeroed first unless
        RZ_FLAG_ACCUMULATE_DH (fp32 reductions whose order is not fixed, as in rz_linear_backward_weight);
      bias_grad[g,:] = sum over the rows of group g of dY[r,:], fp32 [groups, N], zeroed first (fp32 reductions too).
-   For a layer with a ReLU, Y is its saved output and dY counts only where Y > 0; dYm [M,N] receives the masked gradient (its rows of
+   For a layer with a ReLU, Y is its saved output and dY counts except where Y <= 0; dYm [M,N] receives the masked gradient (its rows of
    no group are not written).  X may be NULL when dH is, hashed and copies when dX is.  rz_plan()'s TCGEN05 path wants X, dY, dYm
    and dX 16-byte aligned. */
 int rz_grouped_backward(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const void *dY, const void *Y,

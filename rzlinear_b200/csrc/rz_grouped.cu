@@ -266,7 +266,7 @@ rz_grouped_prepare_kernel(const T *__restrict__ dY, const T *__restrict__ Y, T *
             const Pack y = *reinterpret_cast<const Pack *>(Y + at);
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (!(to_f32<T>(y.e[i]) > 0.f)) g.e[i] = T(0.f);
+                if (to_f32<T>(y.e[i]) <= 0.f) g.e[i] = T(0.f);   // (not for a NaN: its gradient goes on)
         }
         if (dYm) *reinterpret_cast<Pack *>(dYm + at) = g;
 #pragma unroll

@@ -206,7 +206,7 @@ rz_simt_kernel(const T *__restrict__ A, const T *__restrict__ B2, const float *_
                     float v = acc[i][j] * alpha;
                     if (OP == 0) {
                         if (bias) v += bias[c];
-                        if (relu) v = fmaxf(v, 0.f);
+                        if (relu) v = GROUPED ? (v < 0.f ? 0.f : v) : fmaxf(v, 0.f);   // (grouped: a NaN stays one)
                     }
                     out[(size_t)r * cols + c] = from_f32<T>(v);
                 }

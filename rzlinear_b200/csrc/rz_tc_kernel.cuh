@@ -762,7 +762,7 @@ rz_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ C
                         }
                         if (p.relu) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) f[j] = fmaxf(f[j], 0.f);
+                            for (int j = 0; j < 32; ++j) f[j] = GROUPED ? (f[j] < 0.f ? 0.f : f[j]) : fmaxf(f[j], 0.f);   // (grouped: a NaN stays one)
                         }
                     }
                     uint8_t *stage = reinterpret_cast<uint8_t *>(scratch);

@@ -348,7 +348,7 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
                     float f = __uint_as_float(v[j]) * p.alpha + bias;
-                    if (p.relu) f = fmaxf(f, 0.f);
+                    if (p.relu && f < 0.f) f = 0.f;   // (a NaN stays one)
                     h[j] = __bfloat16_as_ushort(__float2bfloat16_rn(f));
                 }
                 if (rows == 32) {

@@ -215,6 +215,21 @@ def test_relu_masks_the_gradient_with_the_saved_output(rz, dtype, K, N, BK, BN):
 
 
 @pytest.mark.parametrize("dtype,K,N,BK,BN", [(BF16, 256, 320, 32, 64), (F32, 37, 53, 8, 5), (F32, 128, 128, 32, 32)])
+def test_relu_lets_nan_through(rz, dtype, K, N, BK, BN):
+    case = Case([40, 0, 90], K, N, BK, BN, 0, dtype, bias=True, relu=True)
+    clean = case.call(rz, BK, BN, 0)
+    case.x[5, 3] = float("nan")
+    y, dx, dh, db = case.call(rz, BK, BN, 0)
+    assert bool(y[5].isnan().all())
+    keep = torch.arange(case.M, device=DEV) != 5
+    assert torch.equal(y[keep], clean[0][keep]) and torch.equal(dx[keep], clean[1][keep])
+    # like torch.relu: the gradient of a NaN goes on (and group 0's weights learn of it)
+    wanted = case.g[5].double() @ (case.h.bfloat16() if dtype == BF16 else case.h).double()[case.words[0]].T * case.alpha
+    assert float((dx[5].double() - wanted).norm() / wanted.norm()) < 2.0**-7
+    assert bool(dh.isnan().any()) and bool(db.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype,K,N,BK,BN", [(BF16, 256, 320, 32, 64), (F32, 37, 53, 8, 5), (F32, 128, 128, 32, 32)])
 def test_each_group_is_a_linear_layer(rz, dtype, K, N, BK, BN):
     # group g's weight is an RzLinear's whose R1 and R4 are advanced by its first tile row
     case = Case([70, 0, 130, 5], K, N, BK, BN, 1, dtype)
