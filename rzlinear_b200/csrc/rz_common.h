@@ -84,14 +84,13 @@ int rz_tc_wait_selftest(long long limit_cycles, cudaStream_t stream);
 
 // rows picked by an index (rz_rows.cu): M = rows or tokens, K = table rows, N = row length
 size_t rz_rows_sort_scratch(int64_t rows, int64_t bins);
-int rz_rows_sort_max_bins();
 int rz_rows_sort(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order, int32_t *offsets, void *scratch, cudaStream_t stream);
 int rz_rows_embedding(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const float *hashed, void *out, void *plan);
 size_t rz_rows_embedding_plan(const rz_problem *pb);
 int rz_rows_embedding_grad(const RzLaunchCtx &c, const int64_t *ids, int64_t padding, const void *dout, float *dH, const void *plan);
 
 // products grouped by row (rz_grouped.cu): pb->M rows in `groups` consecutive groups given by offsets[groups + 1] on the device
-constexpr int RZ_GROUPS_MAX = 4096;
+constexpr int RZ_GROUPS_MAX = RZ_GROUPS_LIMIT;
 size_t rz_grouped_workspace(const rz_problem *pb, int groups, bool tc);
 int rz_grouped_run_forward(const RzLaunchCtx &c, int groups, const int32_t *offsets, const void *X, const float *hashed, const void *copies,
                            const float *bias, void *Y, void *ws, bool tc);

@@ -46,7 +46,7 @@ __device__ __forceinline__ bool live_id(int64_t id, uint32_t V, int64_t padding)
 // reproducible, rank without any atomic on a shared counter.
 constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32, SORT_ITEMS = 4;
 constexpr int SORT_TILE = SORT_THREADS * SORT_ITEMS;
-constexpr int SORT_MAX_BINS = 1024, SORT_MAX_BLOCKS = 148;
+constexpr int SORT_MAX_BINS = RZ_SORT_MAX_BINS, SORT_MAX_BLOCKS = 148;
 
 // Lanes whose `bits` low key bits equal this lane's, one vote per bit.
 __device__ __forceinline__ uint32_t same_key(uint32_t key, int bits)
@@ -760,8 +760,6 @@ size_t rz_rows_sort_scratch(int64_t rows, int64_t bins)
     const uint32_t blocks = rows > 0 ? sort_blocks(rows, &per) : 1;
     return blocks <= 1 ? 0 : sizeof(uint32_t) * (size_t)blocks * (size_t)(bins + 1);
 }
-
-int rz_rows_sort_max_bins() { return SORT_MAX_BINS; }
 
 int rz_rows_sort(const int64_t *keys, int64_t rows, int64_t bins, int32_t *order, int32_t *offsets, void *scratch, cudaStream_t stream)
 {

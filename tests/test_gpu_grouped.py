@@ -473,6 +473,39 @@ def test_offsets_beyond_32_bits(rz):
     assert float((dh.double() - total).norm() / total.norm()) < 1e-5      # the framework's bar for fp32 results
 
 
+@pytest.mark.parametrize("dtype,K,N,BK,BN", [(BF16, 256, 320, 32, 64), (F32, 128, 160, 32, 32)])
+def test_call_options_give_the_same_bits(rz, rzlib, dtype, K, N, BK, BN):
+    # small whole numbers: every product and sum is exact in fp32 (and rounded once to bf16), whatever computes them in whatever order
+    case = Case([300, 0, 33, 1], K, N, BK, BN, 1, dtype, before=2, behind=3)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    whole = lambda t: torch.randint(-2, 3, t.shape, generator=g, device=DEV).to(t.dtype)
+    x, dy, h, bias = whole(case.x), whole(case.g), whole(case.h), torch.randint(-2, 3, (4, N), generator=g, device=DEV).float()
+    io, prec = (rzlib.BF16, rzlib.PREC_BF16) if dtype == BF16 else (rzlib.F32, rzlib.PREC_FP32)
+    pb = rzlib.make_problem(case.M, K, N, case.H, BK, BN, case.R, 1, io, prec, alpha=0.5)
+    assert rzlib.plan(pb, 0) == rzlib.PATH_TCGEN05
+
+    def run(pb, want=("dx", "dh", "db"), dh=None):
+        copies_bytes, ws_bytes = rzlib.grouped_sizes(pb, 4)
+        copies = torch.empty(copies_bytes, dtype=torch.uint8, device=DEV) if copies_bytes else None
+        if copies is not None:
+            rzlib.shadow_refresh(pb, h, copies)
+        y, ws = torch.empty_like(dy), torch.empty(ws_bytes, dtype=torch.uint8, device=DEV)
+        rzlib.grouped_forward(pb, 4, case.offsets, x, h, copies, bias, y, ws)
+        out = {"dx": torch.empty_like(x), "dh": torch.empty_like(h) if dh is None else dh, "db": torch.empty_like(bias)}
+        rzlib.grouped_backward(pb, 4, case.offsets, x, dy, None, h, copies, None, *(out[k] if k in want else None for k in ("db", "dx", "dh")), ws)
+        return {"y": y, **{k: out[k] for k in want}}
+
+    first = run(pb)
+    assert float(first["dh"].abs().max()) > 0 and float(first["dx"].abs().max()) > 0
+    others = [run(rzlib.with_fields(pb, flags=rzlib.FLAG_FORCE_SIMT)), run(rzlib.with_fields(pb, sm_reserve=100)),
+              run(pb, ("dx",)), run(pb, ("dh",)), run(pb, ("db",)), run(pb, ("dh", "db"))]
+    for other in others:
+        for k, v in other.items():
+            assert torch.equal(v, first[k]), k
+    twice = run(rzlib.with_fields(pb, flags=rzlib.FLAG_ACCUMULATE_DH), dh=first["dh"].clone())["dh"]
+    assert torch.equal(twice, 2 * first["dh"])
+
+
 def test_views_that_begin_anywhere(rz):
     case = Case([70, 0, 130, 5], 256, 320, 32, 64, 1, BF16)
     clean = case.call(rz, 32, 64, 1)
