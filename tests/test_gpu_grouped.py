@@ -484,14 +484,14 @@ def test_call_options_give_the_same_bits(rz, rzlib, dtype, K, N, BK, BN):
     pb = rzlib.make_problem(case.M, K, N, case.H, BK, BN, case.R, 1, io, prec, alpha=0.5)
     assert rzlib.plan(pb, 0) == rzlib.PATH_TCGEN05
 
-    def run(pb, want=("dx", "dh", "db"), dh=None):
+    def run(pb, want=("dx", "dh", "db"), dh=None, db=None):
         copies_bytes, ws_bytes = rzlib.grouped_sizes(pb, 4)
         copies = torch.empty(copies_bytes, dtype=torch.uint8, device=DEV) if copies_bytes else None
         if copies is not None:
             rzlib.shadow_refresh(pb, h, copies)
         y, ws = torch.empty_like(dy), torch.empty(ws_bytes, dtype=torch.uint8, device=DEV)
         rzlib.grouped_forward(pb, 4, case.offsets, x, h, copies, bias, y, ws)
-        out = {"dx": torch.empty_like(x), "dh": torch.empty_like(h) if dh is None else dh, "db": torch.empty_like(bias)}
+        out = {"dx": torch.empty_like(x), "dh": torch.empty_like(h) if dh is None else dh, "db": torch.empty_like(bias) if db is None else db}
         rzlib.grouped_backward(pb, 4, case.offsets, x, dy, None, h, copies, None, *(out[k] if k in want else None for k in ("db", "dx", "dh")), ws)
         return {"y": y, **{k: out[k] for k in want}}
 
@@ -499,6 +499,7 @@ def test_call_options_give_the_same_bits(rz, rzlib, dtype, K, N, BK, BN):
     assert float(first["dh"].abs().max()) > 0 and float(first["dx"].abs().max()) > 0
     others = [run(rzlib.with_fields(pb, flags=rzlib.FLAG_FORCE_SIMT)), run(rzlib.with_fields(pb, sm_reserve=100)),
               run(pb, ("dx",)), run(pb, ("dh",)), run(pb, ("db",)), run(pb, ("dh", "db"))]
+    others += [run(pb, ("db",), db=torch.empty(4 * N + 1, device=DEV)[1:].view(4, N))]     # (begins at an odd word)
     for other in others:
         for k, v in other.items():
             assert torch.equal(v, first[k]), k
