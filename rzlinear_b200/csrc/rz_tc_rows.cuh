@@ -333,9 +333,11 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
             if (!ok) break;
             tc_fence_after();
             const uint32_t acc = tmem_base + ((q * 32u) << 16) + (buf * RB + rblk) * NMAX;
-            const uint32_t chunks = (row_end - row + 31) / 32;
+            // A warp whose columns all lie past the matrix stores nothing, and must not turn its tiles over either: the wait below lets the
+            // newest store go on reading its tile, which is right only while every turn goes with a store.
+            const uint32_t chunks = cbase < p.cols ? (row_end - row + 31) / 32 : 0u;
             uint32_t next[32];
-            tmem_ld_32x32(acc, next);
+            if (chunks) tmem_ld_32x32(acc, next);
 #pragma unroll 1
             for (uint32_t c = 0; c < chunks; ++c) {
                 uint32_t v[32];
@@ -360,7 +362,7 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
                     for (int j = 0; j < 32; ++j) tile[j * 32 + lane] = h[j];
                     fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0 && cbase < p.cols) {
+                    if (lane == 0) {
                         tma_store_2d(&mapC, smem_u32(tile), (int32_t)cbase, (int32_t)r0);   // (columns past the matrix are clipped)
                         bulk_commit_group();
                     }
