@@ -90,7 +90,10 @@ rz_tc_rows_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constan
     constexpr int NBUF = 2 * RB * NMAX <= 512 ? 2 : 1;
     constexpr int EPI_WARPS = 4 * RB;
     constexpr uint32_t N_STEP = 16 * CTAS;                    // MMA N granularity
-    static_assert(STAGES >= 3, "ring");
+    // A slot's fills come from different producers, and one bit of the phase tells the producer of stage c that stage c - STAGES has been
+    // read.  The bit is right only if stage c - 2 STAGES has been read before it is looked at.  What the producer knows is that stage
+    // c - ROWS_PRODUCERS - STAGES, which its own last stage waited for, has; stages are read in their order.
+    static_assert(STAGES >= ROWS_PRODUCERS, "a producer must not be two phases ahead of a slot");
     static_assert(RB * NMAX <= 512 && NMAX % 32 == 0, "TMEM columns");
 
     extern __shared__ uint8_t smem_raw[];
