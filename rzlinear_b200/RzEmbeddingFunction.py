@@ -9,7 +9,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .RzLinearFunction import DEFAULT_CONFIG, RzConfig
 from .impl import launchers
-from .RzGroupedLinearFunction import _as
+from .RzGroupedLinearFunction import _as, _constant
 from .rows import _index_view
 
 
@@ -47,7 +47,7 @@ class RzEmbeddingFunction(torch.autograd.Function):
     @classmethod
     def apply(cls, *args):
         # nothing to differentiate: the lookup alone, without the autograd machinery (most of a short lookup's time)
-        if not (torch.is_grad_enabled() and args[1].requires_grad):
+        if _constant(args[1]):
             with torch.no_grad():
                 return _lookup(*args, *(None,) * (9 - len(args)), False)[0]
         return super().apply(*args, *(None,) * (9 - len(args)))

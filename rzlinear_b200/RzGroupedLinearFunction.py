@@ -4,6 +4,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -36,6 +37,15 @@ def _operand(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _constant(*tensors) -> bool:
+    """None of the tensors wants a gradient or carries a tangent (forward-mode derivatives are left to autograd, which refuses them)."""
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and ((grad and t.requires_grad) or unpack_dual(t).tangent is not None):
+            return False
+    return True
+
+
 def _product(input, hashed_weight, random_numbers, offsets, output_dim, init_factor, config, bias):
     """(output in the compute dtype, int32 offsets, problem, groups, shifted copies): the forward pass and what the backward wants of it."""
     cfg = config if config is not None else DEFAULT_CONFIG
@@ -65,7 +75,7 @@ class RzGroupedLinearFunction(torch.autograd.Function):
     @classmethod
     def apply(cls, *args):
         # nothing to differentiate: the product alone, without the autograd machinery
-        if not (torch.is_grad_enabled() and any(a.requires_grad for a in (args[0], args[1], *args[7:]) if a is not None)):
+        if _constant(args[0], args[1], *args[7:]):
             with torch.no_grad():
                 out = _product(*args, *(None,) * (8 - len(args)))[0]
                 return out if out.dtype == args[0].dtype else out.to(args[0].dtype)
