@@ -71,9 +71,9 @@ class RzEmbeddingFunction(torch.autograd.Function):
             Returns:
                 output (Tensor): ids.shape + (embedding_dim).  An id outside [0, num_embeddings) gives zeros and no gradient.
         '''
-        out, index, pb, padding, ctx.plan = _lookup(ids, hashed_weight, random_numbers, num_embeddings, embedding_dim, init_factor,
-                                                    config, padding_idx, out_dtype, ctx.needs_input_grad[1])
-        ctx.save_for_backward(index)
+        out, index, pb, padding, plan = _lookup(ids, hashed_weight, random_numbers, num_embeddings, embedding_dim, init_factor,
+                                                config, padding_idx, out_dtype, ctx.needs_input_grad[1])
+        ctx.save_for_backward(index, plan)
         ctx.pb, ctx.padding = pb, padding
         ctx.weight_shape, ctx.weight_dtype = hashed_weight.shape, hashed_weight.dtype
         return out
@@ -81,13 +81,13 @@ class RzEmbeddingFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        index, = ctx.saved_tensors
+        index, plan = ctx.saved_tensors
         weight_grad = None
         if ctx.needs_input_grad[1]:
             grad = _as(grad, torch.bfloat16 if ctx.pb.io_dtype == _lib.BF16 else torch.float32).contiguous()
             dh = torch.empty((ctx.pb.H,), device=index.device, dtype=torch.float32)
             if index.numel():
-                _lib.embedding_backward(ctx.pb, index, ctx.padding, grad, dh, ctx.plan)   # zeroes dh first
+                _lib.embedding_backward(ctx.pb, index, ctx.padding, grad, dh, plan)   # zeroes dh first
             else:
                 dh.zero_()
             weight_grad = _as(dh, ctx.weight_dtype, ctx.weight_shape)

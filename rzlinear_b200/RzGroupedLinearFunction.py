@@ -102,16 +102,17 @@ class RzGroupedLinearFunction(torch.autograd.Function):
         out, off, pb, groups, copies = _product(input, hashed_weight, random_numbers, offsets, output_dim, init_factor, config, bias)
         # (the saved output keeps the compute dtype: the backward masks with it)
         relu = bool(pb.flags & _lib.FLAG_RELU)
-        ctx.save_for_backward(input, hashed_weight, off, out if relu else None)
+        if copies is not None:   # the backward reads the weights the forward saw; a longer buffer has a linear layer's workspace behind them
+            copies = copies[:_lib.grouped_sizes(pb, groups)[0]]
+        ctx.save_for_backward(input, hashed_weight, off, out if relu else None, copies)
         ctx.pb, ctx.groups, ctx.relu = pb, groups, relu
-        ctx.copies = copies  # the backward reads the weights the forward saw
         ctx.bias_dtype = None if bias is None else bias.dtype
         return out if out.dtype == input.dtype else out.to(input.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        input, hashed_weight, off, out = ctx.saved_tensors
+        input, hashed_weight, off, out, copies = ctx.saved_tensors
         pb, groups = ctx.pb, ctx.groups
         x = _operand(_compute_view(input))
         M, make = input.shape[0], torch.empty if input.shape[0] else torch.zeros
@@ -121,7 +122,7 @@ class RzGroupedLinearFunction(torch.autograd.Function):
         bias_grad = make((groups, pb.N), device=x.device, dtype=torch.float32) if ctx.needs_input_grad[7] else None
         if M:
             hashed = None if dx is None else launchers._hashed_f32(hashed_weight)
-            _lib.grouped_backward(pb, groups, off, x, grad, out if ctx.relu else None, hashed, ctx.copies,
+            _lib.grouped_backward(pb, groups, off, x, grad, out if ctx.relu else None, hashed, copies,
                                   torch.empty_like(grad) if ctx.relu else None, bias_grad, dx, dh,
                                   torch.empty(_lib.grouped_sizes(pb, groups)[1], dtype=torch.uint8, device=x.device))
         return (_as(dx, input.dtype), _as(dh, hashed_weight.dtype, hashed_weight.shape), None, None, None, None, None,

@@ -1,9 +1,12 @@
 """What the layers that pick rows by an index tell autograd, with the kernels replaced by host functions (no GPU needed)."""
+import weakref
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import rzlinear_b200 as rz
+from rzlinear_b200 import _lib
 from rzlinear_b200.impl import launchers
 
 
@@ -51,3 +54,41 @@ def test_tangents_are_refused_not_dropped(on_the_host, function, make, which, gr
         args[which] = primal.detach()      # without one, inside a level: an ordinary call
         out = function.apply(*args)
         assert forward_ad.unpack_dual(out).tangent is None and float(out.min()) == 1.0
+
+
+class Held:
+    """What a saved-tensor hook keeps of a tensor."""
+
+    def __init__(self, tensor):
+        self.tensor = tensor
+
+
+@pytest.mark.parametrize("function", [rz.RzEmbeddingFunction, rz.RzGroupedLinearFunction])
+@pytest.mark.parametrize("retain", [False, True])
+def test_buffers_of_the_backward_are_saved_tensors(on_the_host, function, retain):
+    # the plan of a lookup and the shifted copies of a grouped product are seen by hooks (offloading, checkpoints), and go when the
+    # backward has run, like all that autograd saves
+    if function is rz.RzEmbeddingFunction:
+        tokens, V, D = 4100, 1000, 1024                       # long enough for a plan
+        weight = torch.randn(V * D // 16).requires_grad_()
+        args = [torch.randint(0, V, (tokens,)), weight, rz.RzEmbedding(V, D)._random_numbers, V, D, 1.0]
+        nbytes = 8 * tokens
+    else:
+        args = grouped_call()
+        weight = args[1]
+        pb = launchers.cached_problem(6, 128, 64, weight.numel(), args[2], 32, 64, torch.float32, False, 1.0, 1)
+        nbytes = _lib.grouped_sizes(pb, 4)[0] or 1
+    held = weakref.WeakSet()
+
+    def pack(tensor):
+        kept = Held(tensor)
+        held.add(kept)
+        return kept
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda kept: kept.tensor):
+        out = function.apply(*args)
+    assert [k.tensor.numel() for k in held if k.tensor.dtype == torch.uint8] == [nbytes]
+    for _ in range(2 if retain else 1):
+        (grad,) = torch.autograd.grad(out, weight, torch.ones_like(out), retain_graph=retain)
+        assert float(grad.min()) == 1.0
+    assert bool(len(held)) == retain
