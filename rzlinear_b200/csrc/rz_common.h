@@ -105,7 +105,7 @@ int rz_simt_grouped_backward_weight(const RzLaunchCtx &c, const RzGroupPieces &p
 
 // tensor-core launches of a grouped operation (rz_tc_grouped.cu)
 struct RzTcGroupPlan {
-    int ctas, rb, nc, ew;   // block shape (bf16 products: nc = most rows of a block)
+    int ctas, rb, nc;       // block shape (bf16 products: nc = most rows of a block)
     uint32_t step;          // most rows of a piece
     bool even;              // a group's pieces are equal
 };

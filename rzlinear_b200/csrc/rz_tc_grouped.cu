@@ -180,7 +180,7 @@ RzTcGroupPlan rows_plan(const rz_problem *pb, int groups, int op)
         const double time = waves * (stages * (s.fixed + s.per_row * mean / pieces) + besides);
         if (best_time < 0.0 || time < best_time || i == forced) {
             best_time = i == forced ? 0.0 : time;
-            best.ctas = s.ctas, best.rb = s.rb, best.nc = s.nmax, best.ew = 1, best.step = (uint32_t)s.nmax, best.even = true;
+            best.ctas = s.ctas, best.rb = s.rb, best.nc = s.nmax, best.step = (uint32_t)s.nmax, best.even = true;
         }
     }
     return best;
@@ -280,7 +280,7 @@ RzTcGroupPlan rz_tc_grouped_plan(const rz_problem *pb, int groups, int op)
     const double used = (double)(pb->M < groups ? pb->M : groups), mean = (double)pb->M / used;
     const int64_t cols = op == RZ_OP_FORWARD ? pb->N : pb->K;
     const int sms = usable_sms(pb);
-    RzTcGroupPlan best = {1, 1, 64, 4, 128, false};
+    RzTcGroupPlan best = {1, 1, 64, 128, false};
     double best_time = -1.0;
     const int forced = forced_shape();
     for (int i = 0; i < 5; ++i) {
@@ -313,7 +313,7 @@ RzTcGroupPlan rz_tc_grouped_plan(const rz_problem *pb, int groups, int op)
         const double time = waves * stages * (double)(s.rb * s.nc) / s.speed;
         if (best_time < 0.0 || time < best_time || i == forced) {
             best_time = i == forced ? 0.0 : time;
-            best.ctas = s.ctas, best.rb = s.rb, best.nc = s.nc, best.ew = dw && !split ? (s.rb == 2 ? 2 : 4) : 1, best.step = step;
+            best.ctas = s.ctas, best.rb = s.rb, best.nc = s.nc, best.step = step;
         }
     }
     return best;
