@@ -1,5 +1,5 @@
-"""Grouped products where block follows block quickly: many blocks a CTA, two or three contraction stages, last column blocks that lie
-mostly past the matrix.
+"""Grouped products at their edges: where block follows block quickly (many blocks a CTA, two or three contraction stages, last column
+blocks that lie mostly past the matrix), as many groups as there may be, few rows, 64-bit activations.
 
 Tolerances: none.  Activations, weights, gradients and bias are small whole numbers, so every product and sum is exact in fp32 (at most
 4 * 16384 * 16 / 2 < 2^24 in magnitude) and an output is rounded at most once: the tensor-core kernels and the FMA kernels give the same
@@ -78,3 +78,40 @@ def test_blocks_in_quick_succession(rz, rzlib, knob, K, N, shape):
         for name, got, exact in zip(("output", "input gradient", "hashed gradient", "bias gradient"), case(), want):
             assert torch.equal(got, exact), name
     assert rzlib.device_status()[0] == 0
+
+
+def agree(case, repeats=2):
+    want = case(simt=True)
+    for _ in range(repeats):
+        for name, got, exact in zip(("output", "input gradient", "hashed gradient", "bias gradient"), case(), want):
+            assert torch.equal(got, exact), name
+    assert case.lib.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("kind", ["few each", "last alone", "none"])
+def test_as_many_groups_as_there_may_be(rz, rzlib, kind):
+    sizes = np.random.RandomState(2).randint(0, 4, 4096) if kind == "few each" else np.zeros(4096, dtype=np.int64)
+    if kind == "last alone":
+        sizes[-1] = 100
+    agree(Whole(rzlib, sizes, 64, 72, behind=5))
+
+
+@pytest.mark.parametrize("shape", [None, 1, 2, 3, 4, 5])
+@pytest.mark.parametrize("sizes", [[64], [1], [0, 0, 37, 0], [5, 0, 60]])
+def test_few_rows_in_one_or_two_groups(rz, rzlib, knob, sizes, shape):
+    if shape is not None:
+        knob("RZ_TC_CONFIG", shape)
+    agree(Whole(rzlib, sizes, 1096, 648, BK=64, BN=128))
+
+
+def test_double_activations_are_computed_in_32_bits(rz):
+    layer = rz.RzGroupedLinear(3, 128, 96, compress_ratio=0.5, block_size_n=32).to(DEV)
+    off = torch.tensor([0, 30, 30, 77], device=DEV, dtype=torch.int32)
+    x = torch.randn(80, 128, device=DEV).double().requires_grad_()
+    y = layer(x, off)
+    assert y.dtype == torch.float64 and torch.equal(y, layer(x.float(), off).double())
+    g = torch.randn_like(y)
+    (dx,) = torch.autograd.grad(y, x, g)
+    xf = x.detach().float().requires_grad_()
+    (dxf,) = torch.autograd.grad(layer(xf, off), xf, g.float())
+    assert dx.dtype == torch.float64 and torch.equal(dx, dxf.double())
