@@ -217,7 +217,8 @@ int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padd
    empty.  Rows before offsets[0] and behind the last offset belong to no group: their results are zeros and they add to no gradient.
    Offsets outside [0, M] count as the nearer end and an offset below an earlier one as that one, so no call reads or writes out of
    range.  1 <= groups <= RZ_GROUPS_LIMIT (RZ_ERR_TOO_LARGE beyond), groups * ceil(K/BK) * BK < 2^31.  Shapes, types and precisions are
-   rz_linear_forward's, and rz_plan() says which kernels run (fp32 precision with K or N above 14336 runs the FMA kernels here).
+   rz_linear_forward's, and rz_plan() says which kernels run (fp32 precision with K or N above 14336 runs the FMA kernels here).  bf16
+   precision on the tensor cores reads the array rounded to bf16, as there; the FMA kernels read it as it is.
 
    `copies`: the shifted copies that rz_shadow_refresh writes (rz_grouped_copies_bytes() of them, 0 on the SIMT path; a shadow
    buffer of rz_linear_forward with the same H and precision serves too); only read, so calls may share them.  `workspace`
@@ -226,8 +227,8 @@ int rz_embedding_backward(const rz_problem *pb, const int64_t *ids, int64_t padd
 size_t rz_grouped_copies_bytes(const rz_problem *pb);
 size_t rz_grouped_workspace_bytes(const rz_problem *pb, int64_t groups);
 
-/* Y[r,:] = alpha * X[r,:] . W_g (+ bias[g,:], fp32 [groups, N], may be NULL) (+ ReLU with RZ_FLAG_RELU, which lets a NaN through) for r in
-   group g.  fp32 precision on the tensor cores: an infinite operand gives NaN. */
+/* Y[r,:] = alpha * X[r,:] . W_g (+ bias[g,:], fp32 [groups, N], may be NULL) (+ ReLU with RZ_FLAG_RELU, which lets a NaN through, where
+   rz_linear_forward's turns it into 0) for r in group g.  fp32 precision on the tensor cores: an infinite operand gives NaN. */
 int rz_grouped_forward(const rz_problem *pb, int64_t groups, const int32_t *offsets, const void *X, const float *hashed,
                        const void *copies, size_t copies_bytes, const float *bias, void *Y, void *workspace, size_t workspace_bytes,
                        void *stream);

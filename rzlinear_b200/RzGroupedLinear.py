@@ -3,6 +3,8 @@
 No counterpart in the reference, whose only layer is RzLinear.  The groups' input_dim x output_dim weights stand one below the other
 in one virtual matrix of the same definition as RzLinear's, every one beginning with a new tile row: group g's weight is that
 of an RzLinear layer whose random numbers R[1] and R[4] are advanced by g * ceil(input_dim / block_size_k) times R[3] and R[7].
+As there, products of bfloat16 activations on the tensor cores read the hashed array rounded to bfloat16; sums are float32.  Unlike
+RzLinear's, the fused ReLU lets a NaN through (forward and backward, like torch.relu); RzLinear's turns it into 0.
 """
 from __future__ import annotations
 

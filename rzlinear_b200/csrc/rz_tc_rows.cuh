@@ -12,8 +12,11 @@
 // What a stage costs, measured with all weights in L2: a row of a weight box starts at a multiple of
 // 16 bytes and so covers two cache lines, about 4.5 clocks of the TMA unit; an aligned row of X costs 1.8.  A stage of 128 weight
 // columns takes 650 clocks plus one for each row of X, a stage of 2 x 128 takes 1140 plus 2.4.
-// Roles, ring, bounded waits and hash tables of the producers are those of rz_tc_kernel.cuh, except that four warps produce.  Accumulator rows are weight columns, so
-// an epilogue thread owns one output column of 32 rows: bias is one value a thread, and 32 rows x 32 columns are transposed by
+// The weights come from the shifted copies, which hold the fp32 array rounded to bf16 (at most 2^-8 of a weight; in a product it shows as
+// 1.7e-3 of the result, root mean square, as much as rounding the result to bf16 does).  It is the linear layer's choice too: keeping
+// the lost bits would take a second MMA and twice the weight loads, which are what bounds few rows.  Sums are fp32.
+// Roles, ring, bounded waits and hash tables of the producers are those of rz_tc_kernel.cuh, except that four warps produce.  Accumulator
+// rows are weight columns, so an epilogue thread owns one output column of 32 rows: bias is one value a thread, and 32 rows x 32 columns are transposed by
 // 2-byte stores into a tile of 64-byte rows (a warp's lanes are neighbours in the row: no bank conflicts), which a bulk tensor
 // store writes out; rows of a ragged end are stored one by one, since the rows behind belong to the next group.
 #pragma once
